@@ -46,9 +46,10 @@ __device__ __forceinline__ float scaled_clamp(float v, float inv_or_scale_div, f
   return (q != q) ? q : fminf(fmaxf(q, -limit), limit);
 }
 
-// v / scale for many v and one scale: a reciprocal computed once, then per element one multiply and one
-// Newton correction whose residual is exact under FMA; the quotient is the correctly rounded one (what the
-// division instruction sequence computes), at three instructions instead of a dozen.  +-inf and NaN pass through.
+// v / scale for many v and one scale: Markstein's correction of a quotient estimate (P. Markstein, "Computation of
+// elementary functions on the IBM RISC System/6000 processor", 1990).  With y = RN(1 / scale) and q = RN(v y), the
+// residual r = v - q scale is exact under FMA and RN(q + r y) is the correctly rounded quotient: the reciprocal is
+// computed once, each value costs three instructions.  +-inf and NaN pass through.
 struct Divisor {
   float scale, inv;
 };
