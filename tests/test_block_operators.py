@@ -1,0 +1,565 @@
+"""Routing around the expert linear and the RMS norms around a block: values, gradients, edge cases and refusals.
+
+Every case runs on the CPU path and, marked ``gpu``, on the kernels, against the 64-bit oracles of ``block_oracles.py``
+within the bounds derived there; whole numbers have to be equal.
+"""
+import math
+
+import pytest
+import torch
+
+import block_oracles as oracle
+from viola_b200 import nn, ops
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(params=DEVICES)
+def device(request):
+    return request.param
+
+
+def randn(seed, *shape, dtype=FP32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------------------ router
+ROUTES = [  # tokens, experts, top_k, dtype, bias, padding, normalize, levels (0: continuous logits, else that many values)
+    (1, 1, 1, FP32, False, 0, True, 0),
+    (1, 8, 2, BF16, False, 0, True, 0),
+    (300, 3, 2, FP32, True, 0.2, False, 0),
+    (300, 4, 4, FP16, False, 0, True, 3),
+    (150, 5, 3, BF16, True, 0, True, 2),
+    (133, 8, 2, FP32, True, 0.3, False, 4),
+    (70, 16, 5, BF16, False, 0.5, True, 0),
+    (40, 17, 4, FP16, True, 0, False, 3),
+    (33, 32, 32, FP32, False, 0, True, 0),
+    (65, 60, 4, FP16, True, 0.2, False, 0),
+    (37, 64, 6, BF16, True, 0, True, 5),
+    (34, 100, 8, FP32, True, 0.1, True, 0),
+    (35, 128, 1, BF16, False, 0, False, 0),
+    (36, 256, 8, FP32, True, 0.2, True, 0),
+    (5, 300, 7, FP16, False, 0, True, 4),
+    (34, 512, 10, BF16, False, 0, True, 0),
+    (3, 1000, 32, FP32, True, 0, False, 0),
+    (33, 1024, 3, FP16, True, 0, True, 0),
+]
+
+
+def route_inputs(case, seed=0):
+    tokens, experts, top_k, dtype, bias, padding, normalize, levels = case
+    logits = 2.0 * randn(seed, tokens, experts)
+    if levels:
+        logits = (logits.clamp(-2, 2) * levels / 4).round()
+    mask = None
+    if padding:
+        mask = torch.rand(tokens, generator=torch.Generator().manual_seed(seed + 1)) >= padding
+        logits[~mask] = torch.tensor([math.nan, math.inf, -math.inf])[torch.arange(int((~mask).sum())) % 3][:, None]
+    offset = (0.5 * randn(seed + 2, experts)).round(decimals=1) if bias else None
+    grads = randn(seed + 3, tokens, top_k), 0.7, 0.3
+    return logits.to(dtype), offset, mask, grads
+
+
+@pytest.mark.parametrize("case", ROUTES, ids=str)
+def test_route_values_and_gradients(case, device):
+    tokens, experts, top_k, dtype, _, _, normalize, _ = case
+    logits, bias, mask, (dw, db, dz) = route_inputs(case)
+    expected = oracle.route(logits, top_k, bias=bias, mask=mask, normalize=normalize, dweights=dw, dbalance=db, dz=dz)
+    leaf = logits.to(device).requires_grad_(True)
+    out = nn.route_tokens(leaf, top_k, bias=None if bias is None else bias.to(device),
+                          mask=None if mask is None else mask.to(device), normalize=normalize)
+    assert torch.equal(out.indices.cpu(), expected["indices"]) and torch.equal(out.counts.cpu(), expected["counts"])
+    terms = experts + tokens
+    oracle.assert_matches(out.weights, expected["weights"], terms, "weights")
+    oracle.assert_matches(out.balance_loss, expected["balance"], terms, "balance")
+    oracle.assert_matches(out.z_loss, expected["z"], terms, "z")
+    (out.weights * dw.to(device)).sum().add(db * out.balance_loss).add(dz * out.z_loss).backward()
+    oracle.assert_matches(leaf.grad, expected["dlogits"], terms, "dlogits")
+    # without a graph the same numbers come back
+    again = nn.route_tokens(leaf.detach(), top_k, bias=None if bias is None else bias.to(device),
+                            mask=None if mask is None else mask.to(device), normalize=normalize)
+    for a, b in zip(out, again):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["weights", "balance", "z"])
+def test_route_gradient_of_one_output(which, device):
+    case = (70, 24, 3, FP32, True, 0.2, False, 0)
+    logits, bias, mask, (dw, db, dz) = route_inputs(case, 5)
+    only = dict(dweights=dw if which == "weights" else None, dbalance=db * (which == "balance"), dz=dz * (which == "z"))
+    expected = oracle.route(logits, 3, bias=bias, mask=mask, normalize=False, **only)
+    leaf = logits.to(device).requires_grad_(True)
+    out = nn.route_tokens(leaf, 3, bias=bias.to(device), mask=mask.to(device), normalize=False)
+    {"weights": (out.weights * dw.to(device)).sum(), "balance": db * out.balance_loss, "z": dz * out.z_loss}[which].backward()
+    oracle.assert_matches(leaf.grad, expected["dlogits"], 94, which)
+
+
+def test_route_gradient_against_differences(device):
+    """Central differences of the 64-bit oracle along random directions; the choice is held by wide gaps of a bias."""
+    tokens, experts, top_k = 20, 12, 3
+    logits = randn(1, tokens, experts)
+    bias = 50.0 * torch.arange(experts).float()
+    dw, db, dz = randn(2, tokens, top_k), 1.3, 0.4
+
+    def value(l):
+        r = oracle.route(l, top_k, bias=bias, normalize=True)
+        return float((r["weights"][0] * dw).sum() + db * r["balance"][0] + dz * r["z"][0])
+
+    leaf = logits.to(device).requires_grad_(True)
+    out = nn.route_tokens(leaf, top_k, bias=bias.to(device))
+    ((out.weights * dw.to(device)).sum() + db * out.balance_loss + dz * out.z_loss).backward()
+    for seed in range(3):
+        v = randn(10 + seed, tokens, experts)
+        step = 2.0 ** -7           # truncation step^2 / 6 * third derivative ~ 1e-5 of sums of order 10; the oracle is exact
+        slope = (value(logits + step * v) - value(logits - step * v)) / (2 * step)
+        assert abs(slope - float((leaf.grad.cpu() * v).sum())) < 2e-3
+
+
+def test_route_rows_without_a_choice(device):
+    """Closed experts, rows with nothing open, the type's lowest value, and fewer open experts than choices."""
+    low = torch.finfo(FP32).min
+    logits = torch.tensor([[0.0, 1.0, -math.inf, 2.0], [-math.inf] * 4, [low] * 4, [-math.inf, -math.inf, 5.0, -math.inf],
+                           [low, -math.inf, low, 3.0]])
+    expected = oracle.route(logits, 3, dweights=torch.ones(5, 3) * torch.tensor([1.0, 2.0, 3.0]), dbalance=1.0)
+    leaf = logits.to(device).requires_grad_(True)
+    out = nn.route_tokens(leaf, 3)
+    assert out.indices.tolist() == [[3, 1, 0], [-1, -1, -1], [0, 1, 2], [2, -1, -1], [3, 0, 2]]
+    assert out.indices.cpu().equal(expected["indices"]) and out.counts.cpu().equal(expected["counts"])
+    torch.testing.assert_close(out.weights.cpu(), expected["weights"][0].float(), rtol=1e-6, atol=1e-7)
+    assert out.weights[1].tolist() == [0, 0, 0] and out.weights[3].tolist() == [1, 0, 0]
+    torch.testing.assert_close(out.balance_loss.cpu(), expected["balance"][0].float(), rtol=1e-6, atol=0)
+    ((out.weights * torch.tensor([1.0, 2.0, 3.0], device=device)).sum() + out.balance_loss).backward()
+    torch.testing.assert_close(leaf.grad.cpu(), expected["dlogits"][0].float(), rtol=1e-5, atol=1e-6)
+    assert leaf.grad[1].tolist() == [0, 0, 0, 0]
+
+
+def test_route_all_tokens_masked(device):
+    logits = torch.full((40, 8), math.nan, device=device, requires_grad=True)
+    out = nn.route_tokens(logits, 2, mask=torch.zeros(40, dtype=torch.bool, device=device))
+    assert out.counts.tolist() == [0] * 8 and out.balance_loss.item() == 0 and out.z_loss.item() == 0
+    assert (out.indices == -1).all() and (out.weights == 0).all()
+    (out.weights.sum() + out.balance_loss + out.z_loss).backward()
+    assert (logits.grad == 0).all()
+
+
+def test_route_passes_nan_on_with_indices_in_range(device):
+    logits = randn(0, 6, 8)
+    logits[2, 5], logits[4, 1] = math.nan, math.inf
+    out = nn.route_tokens(logits.to(device), 3, normalize=False)
+    assert ((out.indices >= 0) & (out.indices < 8)).all() and out.indices[2, 0].item() == 5 and out.indices[4, 0].item() == 1
+    assert out.weights[[2, 4]].isnan().any(1).all() and out.weights[[0, 1, 3, 5]].isfinite().all()
+    assert out.balance_loss.isnan() and out.z_loss.isnan() | out.z_loss.isinf()
+
+
+def test_route_shapes_strides_and_no_tokens(device):
+    base = randn(3, 2, 7, 24, dtype=BF16).to(device)
+    logits = base[..., ::2]                                    # strided columns
+    out = nn.route_tokens(logits, 2)
+    flat = nn.route_tokens(logits.reshape(14, 12).contiguous(), 2)
+    assert out.weights.shape == (2, 7, 2) and out.indices.shape == (2, 7, 2)
+    assert torch.equal(out.weights.view(14, 2), flat.weights) and torch.equal(out.balance_loss, flat.balance_loss)
+    rows = randn(4, 5, 40).to(device)[:, 3:35]                 # rows that start off a 16-byte boundary
+    assert torch.equal(nn.route_tokens(rows, 2).weights, nn.route_tokens(rows.contiguous(), 2).weights)
+    empty = torch.empty(0, 12, device=device, requires_grad=True)
+    out = nn.route_tokens(empty, 2)
+    assert out.weights.shape == (0, 2) and out.counts.tolist() == [0] * 12 and out.balance_loss.item() == 0
+    (out.weights.sum() + out.balance_loss).backward()
+    assert empty.grad.shape == (0, 12)
+    one = nn.route_tokens(randn(5, 12).to(device), 2)
+    assert one.weights.shape == (2,)
+
+
+def test_route_refusals(device):
+    logits = torch.zeros(4, 8, device=device)
+    for bad in (dict(top_k=0), dict(top_k=9), dict(top_k=2, bias=torch.zeros(7, device=device)),
+                dict(top_k=2, mask=torch.zeros(3, dtype=torch.bool, device=device)),
+                dict(top_k=2, mask=torch.zeros(4, device=device))):
+        with pytest.raises(ValueError):
+            nn.route_tokens(logits, **bad)
+    with pytest.raises(TypeError):
+        nn.route_tokens(logits.double(), 2)
+    with pytest.raises(TypeError):
+        nn.route_tokens(logits.int(), 2)
+    with pytest.raises(ValueError):
+        nn.route_tokens(torch.zeros(4, 1025, device=device), 2)
+    with pytest.raises(ValueError):
+        nn.route_tokens(torch.zeros(4, 64, device=device), 33)
+    with pytest.raises(ValueError):
+        nn.route_tokens(torch.zeros((), device=device), 1)
+
+
+# ------------------------------------------------------------------------------------------------ dispatch and combine
+PLANS = [(1, 1, 1), (1, 2, 8), (7, 3, 5), (300, 2, 4), (33, 8, 1024), (50, 32, 40), (1000, 5, 17)]   # tokens, top_k, experts
+
+
+def choices(tokens, top_k, experts, dropped=0.2, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    indices = torch.randint(0, experts, (tokens, top_k), generator=g)
+    return torch.where(torch.rand(tokens, top_k, generator=g) < dropped, -1, indices)
+
+
+@pytest.mark.parametrize("case", PLANS, ids=str)
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_plan(case, dtype, device):
+    indices = choices(*case).to(dtype)
+    offsets, positions = oracle.plan(indices, case[2])
+    plan = nn.plan_experts(indices.to(device), case[2])
+    assert torch.equal(plan.offsets.cpu(), offsets) and torch.equal(plan.positions.cpu(), positions)
+
+
+def test_plan_of_many_choices_crosses_blocks(device):
+    """Several blocks with ragged ends, one expert that takes most of it, out-of-range values on both sides."""
+    tokens, top_k, experts = 40001, 3, 9
+    g = torch.Generator().manual_seed(1)
+    indices = torch.randint(-2, experts + 2, (tokens, top_k), generator=g)
+    indices[torch.rand(tokens, top_k, generator=g) < 0.6] = 4
+    plan = nn.plan_experts(indices.to(device), experts)
+    flat = indices.reshape(-1)
+    bins = torch.where((flat >= 0) & (flat < experts), flat, experts)
+    order = torch.argsort(bins, stable=True)
+    counts = torch.bincount(bins, minlength=experts + 1)[:experts]
+    assert plan.offsets.tolist() == [0] + counts.cumsum(0).tolist()
+    expected = torch.full_like(flat, -1)
+    total = int(counts.sum())
+    expected[order[:total]] = torch.arange(total)
+    assert torch.equal(plan.positions.cpu().long().view(-1), expected)
+
+
+def test_plan_without_choices(device):
+    plan = nn.plan_experts(torch.full((5, 2), -1, dtype=torch.int32, device=device), 3)
+    assert plan.offsets.tolist() == [0, 0, 0, 0] and (plan.positions == -1).all()
+    plan = nn.plan_experts(torch.empty(0, 2, dtype=torch.int64, device=device), 3)
+    assert plan.offsets.tolist() == [0, 0, 0, 0] and plan.positions.shape == (0, 2)
+
+
+EXCHANGES = [  # tokens, top_k, experts, width, dtype
+    (1, 1, 1, 1, FP32), (1, 2, 8, 1152, BF16), (5, 3, 4, 7, FP16), (40, 2, 8, 1000, BF16), (33, 4, 6, 771, FP16),
+    (17, 8, 12, 260, FP32), (3, 32, 40, 66, BF16), (9, 2, 3, 4100, BF16), (6, 2, 3, 9001, FP32), (260, 1, 5, 64, FP16),
+]
+
+
+@pytest.mark.parametrize("case", EXCHANGES, ids=str)
+def test_dispatch_values_and_gradients(case, device):
+    tokens, top_k, experts, width, dtype = case
+    indices = choices(tokens, top_k, experts)
+    x = randn(0, tokens, width, dtype=dtype)
+    _, positions = oracle.plan(indices, experts)
+    plan = nn.plan_experts(indices.to(device), experts)
+    leaf = x.to(device).requires_grad_(True)
+    rows = nn.dispatch_tokens(leaf, plan)
+    expected = torch.zeros(tokens * top_k, width, dtype=dtype)
+    for t, j in (positions >= 0).nonzero().tolist():
+        expected[positions[t, j]] = x[t]
+    assert torch.equal(rows.cpu(), expected)               # the rows behind the last are zero
+    grad = randn(1, tokens * top_k, width, dtype=dtype)
+    rows.backward(grad.to(device))
+    back = oracle.combine(grad, torch.ones(tokens, top_k), positions)["out"]
+    oracle.assert_matches(leaf.grad, back, top_k, "dx")
+    assert torch.equal(nn.dispatch_tokens(leaf.detach(), plan), rows)
+
+
+@pytest.mark.parametrize("case", EXCHANGES, ids=str)
+@pytest.mark.parametrize("weight_dtype", [FP32, BF16])
+def test_combine_values_and_gradients(case, weight_dtype, device):
+    tokens, top_k, experts, width, dtype = case
+    indices = choices(tokens, top_k, experts, seed=2)
+    _, positions = oracle.plan(indices, experts)
+    plan = nn.plan_experts(indices.to(device), experts)
+    rows = randn(3, tokens * top_k, width, dtype=dtype)
+    rows[int(plan.offsets[-1]):] = math.nan                # nothing of these rows may be read
+    weights = torch.rand(tokens, top_k, generator=torch.Generator().manual_seed(4)).to(weight_dtype)
+    dout = randn(5, tokens, width, dtype=dtype)
+    expected = oracle.combine(rows.nan_to_num(0), weights, positions, dout)
+    leaf, wleaf = rows.to(device).requires_grad_(True), weights.to(device).requires_grad_(True)
+    out = nn.combine_tokens(leaf, wleaf, plan)
+    oracle.assert_matches(out, expected["out"], top_k, "out")
+    out.backward(dout.to(device))
+    oracle.assert_matches(leaf.grad, expected["drows"], 1, "drows")
+    oracle.assert_matches(wleaf.grad, expected["dweights"], width, "dweights")
+    assert torch.equal(nn.combine_tokens(leaf.detach(), wleaf.detach(), plan), out)
+    # one gradient without the other
+    only_rows, = torch.autograd.grad(nn.combine_tokens(leaf, wleaf.detach(), plan), leaf, dout.to(device))
+    only_weights, = torch.autograd.grad(nn.combine_tokens(leaf.detach(), wleaf, plan), wleaf, dout.to(device))
+    assert torch.equal(only_rows, leaf.grad) and torch.equal(only_weights, wleaf.grad)
+
+
+def test_exchange_shapes_strides_and_no_tokens(device):
+    indices = choices(10, 2, 3).view(2, 5, 2).to(device)
+    plan = nn.plan_experts(indices, 3)
+    base = randn(0, 2, 5, 96, dtype=BF16).to(device)
+    for x in (base[..., :64], base[..., 3:67], base[..., ::2], base.transpose(0, 1).contiguous().transpose(0, 1)[..., :48]):
+        leaf = x.detach().requires_grad_(True)
+        rows = nn.dispatch_tokens(leaf, plan)
+        assert torch.equal(rows, nn.dispatch_tokens(x.contiguous(), plan))
+        out = nn.combine_tokens(rows, torch.ones(2, 5, 2, device=device), plan)
+        assert out.shape == x.shape
+        out.backward(torch.ones_like(out).transpose(0, 1).contiguous().transpose(0, 1))
+        kept = (indices >= 0).sum(-1, keepdim=True)
+        assert torch.equal(leaf.grad, kept.expand(x.shape).to(BF16))
+    rows = randn(1, 21, 64, dtype=BF16).to(device)[1:]        # off the start of its storage
+    weights = randn(2, 2, 2, 5).to(device).permute(1, 2, 0)   # not contiguous
+    assert torch.equal(nn.combine_tokens(rows, weights, plan), nn.combine_tokens(rows.clone(), weights.contiguous(), plan))
+    none = nn.plan_experts(torch.empty(0, 2, dtype=torch.int32, device=device), 3)
+    x = torch.empty(0, 8, device=device, requires_grad=True)
+    out = nn.combine_tokens(nn.dispatch_tokens(x, none), torch.empty(0, 2, device=device), none)
+    assert out.shape == (0, 8)
+    out.sum().backward()
+    assert x.grad.shape == (0, 8)
+
+
+def test_combine_skips_positions_out_of_range(device):
+    """A plan is the caller's data: positions that name no row are passed over, not followed."""
+    plan = nn.ExpertPlan(torch.tensor([0, 4, 9], dtype=torch.int32, device=device),
+                         torch.tensor([[0, 7], [-5, 1], [3, 2 ** 31 - 1]], dtype=torch.int32, device=device))
+    rows = torch.ones(6, 16, device=device, requires_grad=True)
+    out = nn.combine_tokens(rows, torch.ones(3, 2, device=device), plan)
+    assert out[:, 0].tolist() == [1, 1, 1]
+    out.sum().backward()
+    assert rows.grad[[0, 1, 3]].eq(1).all()
+    assert nn.dispatch_tokens(torch.ones(3, 16, device=device), plan)[[0, 1, 3]].eq(1).all()
+
+
+def test_exchange_refusals(device):
+    indices = torch.zeros(4, 2, dtype=torch.int32, device=device)
+    plan = nn.plan_experts(indices, 3)
+    x, rows, weights = torch.zeros(4, 16, device=device), torch.zeros(8, 16, device=device), torch.ones(4, 2, device=device)
+    for bad in (lambda: nn.plan_experts(indices, 0), lambda: nn.plan_experts(indices, 1025),
+                lambda: nn.plan_experts(torch.zeros(4, 33, dtype=torch.int32, device=device), 3),
+                lambda: nn.plan_experts(torch.zeros(4, 0, dtype=torch.int32, device=device), 3),
+                lambda: nn.dispatch_tokens(x[:3], plan), lambda: nn.dispatch_tokens(x[:, :0], plan),
+                lambda: nn.combine_tokens(rows[:7], weights, plan), lambda: nn.combine_tokens(rows, weights[:, :1], plan),
+                lambda: nn.combine_tokens(rows.view(4, 2, 16), weights, plan),
+                lambda: nn.dispatch_tokens(x, nn.ExpertPlan(plan.offsets.long(), plan.positions)),
+                lambda: nn.dispatch_tokens(x, nn.ExpertPlan(plan.offsets, plan.positions.view(-1)))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: nn.plan_experts(indices.float(), 3), lambda: nn.dispatch_tokens(x.double(), plan),
+                lambda: nn.combine_tokens(rows.double(), weights, plan), lambda: nn.combine_tokens(rows, weights.double(), plan)):
+        with pytest.raises(TypeError):
+            bad()
+
+
+# ------------------------------------------------------------------------------------------------------------- norms
+NORMS = [  # batch, tokens, width, stream, branch, weights, gate, scale, post, pre, residual
+    (1, 1, 1, FP32, FP32, True, "shared", "shared", True, True, 1.0),
+    (1, 1, 4096, BF16, BF16, True, None, None, True, True, 1.0),
+    (3, 5, 64, BF16, BF16, True, "sample", "sample", True, True, 0.5),
+    (2, 7, 72, FP32, BF16, True, "sample", "shared", True, True, 1.25),
+    (4, 1, 1152, FP32, BF16, False, "sample", "sample", True, True, 1.0),
+    (2, 33, 1152, FP32, FP16, True, "shared", "sample", True, True, -0.7),
+    (7, 3, 1001, FP16, FP16, True, "sample", None, True, False, 0.5),
+    (2, 9, 771, FP32, FP32, True, None, "sample", False, True, 1.0),
+    (1, 300, 256, BF16, BF16, True, None, None, True, True, 1.0),
+    (300, 2, 40, FP16, FP16, True, "sample", "sample", True, True, 1.0),
+    (2, 3, 2056, FP32, BF16, True, "sample", "sample", True, True, 1.0),
+    (1, 4, 8192, BF16, BF16, True, "shared", None, True, True, 1.4),
+    (2, 2, 8200, FP32, FP32, True, "sample", "sample", True, True, 1.0),
+    (1, 2, 2049, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (1, 3, 16384, FP16, FP16, True, "sample", "sample", True, True, 1.0),
+    (1, 2, 16383, FP32, BF16, True, "shared", "shared", True, True, 1.0),
+    (2, 40, 512, FP32, BF16, False, None, None, True, True, 1.0),
+    (2, 40, 264, BF16, BF16, False, None, None, False, True, 1.0),
+]
+
+
+def norm_inputs(case, seed=0):
+    batch, tokens, width, stream, branch, weights, gate, scale, post, pre, _ = case
+    shape = {"shared": (width,), "sample": (batch, width)}
+    v = dict(x=2 * randn(seed, batch, tokens, width), y=None, weight=None, gate=None, next_weight=None, next_scale=None)
+    v["x"] = v["x"].to(stream)
+    if post:
+        v["y"] = randn(seed + 1, batch, tokens, width, dtype=branch)
+        v["weight"] = 1 + 0.2 * randn(seed + 2, width) if weights else None
+        v["gate"] = 0.5 * randn(seed + 3, *shape[gate]).to(branch) if gate else None
+    if pre:
+        v["next_weight"] = (1 + 0.2 * randn(seed + 4, width)).to(branch) if weights else None
+        v["next_scale"] = 0.3 * randn(seed + 5, *shape[scale]).to(branch) if scale else None
+    dout = randn(seed + 6, batch, tokens, width, dtype=stream) if post else None
+    dh = randn(seed + 7, batch, tokens, width, dtype=branch) if pre else None
+    return v, dout, dh
+
+
+def call_norm(case, v, **kwargs):
+    post, pre, residual = case[8:]
+    if not post:
+        return None, nn.rms_norm_modulate(v["x"], v["next_weight"], v["next_scale"], dtype=case[4], **kwargs)
+    out = nn.rms_norm_residual(v["x"], v["y"], v["weight"], v["gate"], residual_scale=residual, next_norm=pre,
+                               next_weight=v["next_weight"], next_scale=v["next_scale"], **kwargs)
+    return out if pre else (out, None)
+
+
+@pytest.mark.parametrize("case", NORMS, ids=str)
+def test_norm_values_and_gradients(case, device):
+    v, dout, dh = norm_inputs(case)
+    batch, tokens, width = case[:3]
+    expected = oracle.block_norm(**v, residual_scale=case[10], next_norm=case[9], dout=dout, dh=dh)
+    leaves = {n: None if t is None else t.to(device).requires_grad_(True) for n, t in v.items()}
+    out, h = call_norm(case, leaves)
+    outs, grads = [], []
+    for name, t, g in (("out", out, dout), ("h", h, dh)):
+        if t is not None:
+            oracle.assert_matches(t, expected[name], width, name)
+            outs.append(t)
+            grads.append(g.to(device))
+    torch.autograd.backward(outs, grads)
+    for name, leaf in leaves.items():
+        if leaf is not None:
+            assert leaf.grad.dtype == leaf.dtype
+            oracle.assert_matches(leaf.grad, expected["d" + name], width + batch * tokens, "d" + name)
+    plain = call_norm(case, {n: None if t is None else t.detach() for n, t in leaves.items()})
+    for a, b in zip(plain, (out, h)):
+        assert a is None and b is None or torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", ["out", "h"])
+def test_norm_gradient_of_one_output(which, device):
+    case = (3, 5, 200, FP32, BF16, True, "sample", "sample", True, True, 0.8)
+    v, dout, dh = norm_inputs(case, 3)
+    only = dict(dout=dout if which == "out" else None, dh=dh if which == "h" else None)
+    expected = oracle.block_norm(**v, residual_scale=0.8, **only)
+    leaves = {n: t.to(device).requires_grad_(True) for n, t in v.items()}
+    out, h = call_norm(case, leaves)
+    (out if which == "out" else h).backward((dout if which == "out" else dh).to(device))
+    for name, leaf in leaves.items():
+        if "d" + name in expected and not (which == "out" and name.startswith("next")):
+            oracle.assert_matches(leaf.grad, expected["d" + name], 215, "d" + name)
+        else:
+            assert leaf.grad is None or not leaf.grad.any()
+
+
+def test_norm_gradient_against_differences(device):
+    case = (2, 4, 24, FP32, FP32, True, "sample", "sample", True, True, 0.9)
+    v, dout, dh = norm_inputs(case, 9)
+
+    def value(inputs):
+        r = oracle.block_norm(**inputs, residual_scale=0.9)
+        return float((r["out"][0] * dout).sum() + (r["h"][0] * dh).sum())
+
+    leaves = {n: t.to(device).requires_grad_(True) for n, t in v.items()}
+    out, h = call_norm(case, leaves)
+    torch.autograd.backward([out, h], [dout.to(device), dh.to(device)])
+    for seed, name in enumerate(v):
+        direction = randn(20 + seed, *v[name].shape)
+        step = 2.0 ** -8             # truncation step^2 / 6 * third derivative ~ 1e-4 at most; the oracle is exact
+        slope = (value({**v, name: v[name].double() + step * direction}) - value({**v, name: v[name].double() - step * direction})) / (2 * step)
+        assert abs(slope - float((leaves[name].grad.cpu() * direction).sum())) < 5e-3 * max(1.0, abs(slope)), name
+
+
+def test_norm_needs_only_what_is_asked(device):
+    case = (3, 4, 136, BF16, BF16, True, "sample", "sample", True, True, 1.1)
+    v, dout, dh = norm_inputs(case, 4)
+    full = {n: t.detach().to(device).requires_grad_(True) for n, t in v.items()}
+    torch.autograd.backward(call_norm(case, full), [dout.to(device), dh.to(device)])
+    for name in v:
+        some = {n: t.detach().to(device).requires_grad_(n == name) for n, t in v.items()}
+        torch.autograd.backward(call_norm(case, some), [dout.to(device), dh.to(device)])
+        assert torch.equal(some[name].grad, full[name].grad)
+        assert all(t.grad is None for n, t in some.items() if n != name)
+
+
+def test_norm_strides_views_and_broadcast_vectors(device):
+    """Chunks of an adaLN projection, transposed and offset streams, expanded vectors: the same numbers as contiguous copies."""
+    batch, tokens, width = 3, 6, 64
+    ada = randn(0, batch, 6 * width, dtype=BF16).to(device)
+    gate, scale = ada.chunk(6, -1)[2], ada.chunk(6, -1)[4]
+    x = randn(1, tokens, batch, width).to(device).transpose(0, 1)
+    y = randn(2, batch, tokens, width + 3, dtype=BF16).to(device)[..., 3:]
+    w = randn(3, 2 * width).to(device)[::2]
+    views, copies = [], []
+    for make, store in ((lambda t: t, views), (lambda t: t.contiguous(), copies)):
+        for g in (gate, gate[:1].expand(batch, width), gate[0]):
+            leaves = [make(t).detach().requires_grad_(True) for t in (x, y, w, g, w, scale)]
+            out, h = nn.rms_norm_residual(leaves[0], leaves[1], leaves[2], leaves[3], next_norm=True, next_weight=leaves[4],
+                                          next_scale=leaves[5])
+            (out.float().sum() + (h.float() * h.float()).sum()).backward()
+            store += [out, h] + [t.grad for t in leaves]
+    for a, b in zip(views, copies):
+        assert torch.equal(a, b)
+    flat = nn.rms_norm_modulate(x.reshape(-1, width)[0].contiguous())            # one vector
+    assert flat.shape == (width,)
+    per_row = nn.rms_norm_modulate(x.reshape(-1, width), scale=x.reshape(-1, width))  # a 2-D stream: one scale per row
+    assert per_row.shape == (batch * tokens, width)
+
+
+def test_norm_gradient_of_an_expanded_gate(device):
+    """A gate broadcast over the batch outside gets the sum over the samples."""
+    case = (4, 3, 48, FP32, FP32, True, "sample", None, True, False, 1.0)
+    v, dout, _ = norm_inputs(case, 6)
+    leaf = v["gate"][:1].to(device).requires_grad_(True)
+    out = nn.rms_norm_residual(v["x"].to(device), v["y"].to(device), v["weight"].to(device), leaf.expand(4, 48))
+    out.backward(dout.to(device))
+    expected = oracle.block_norm(v["x"], v["y"], v["weight"], v["gate"][0], next_norm=False, dout=dout)["dgate"]
+    oracle.assert_matches(leaf.grad[0], expected, 48 + 12 + 4, "gate")
+
+
+def test_norm_zero_rows_and_extreme_values(device):
+    x = torch.zeros(2, 3, 40, device=device, requires_grad=True)
+    y = torch.zeros(2, 3, 40, device=device, requires_grad=True)
+    out, h = nn.rms_norm_residual(x, y, next_norm=True)
+    assert (out == 0).all() and (h == 0).all()
+    (out + h).sum().backward()
+    # by the formula: du = 1 + 1 / sqrt(eps), dx = du, dy = du / sqrt(eps)
+    root = (1e-6) ** -0.5
+    torch.testing.assert_close(x.grad, torch.full_like(x, 1 + root), rtol=1e-5, atol=0)
+    torch.testing.assert_close(y.grad, torch.full_like(y, (1 + root) * root), rtol=1e-5, atol=0)
+    big = torch.full((1, 1, 64), 3e4, dtype=FP16, device=device)          # squares overflow fp16, not fp32
+    torch.testing.assert_close(nn.rms_norm_modulate(big), torch.ones_like(big), rtol=0, atol=0)
+    bad = torch.ones(1, 2, 64, device=device)
+    bad[0, 1, 3] = math.nan
+    res = nn.rms_norm_modulate(bad)
+    assert res[0, 0].isfinite().all() and res[0, 1].isnan().all()          # a row's NaN stays in its row
+
+
+def test_norm_without_rows(device):
+    for shape in ((0, 4, 32), (2, 0, 32)):
+        x, y = (torch.empty(shape, device=device, requires_grad=True) for _ in range(2))
+        w = torch.ones(32, device=device, requires_grad=True)
+        gate = torch.ones(shape[0], 32, device=device, requires_grad=True)
+        out, h = nn.rms_norm_residual(x, y, w, gate, next_norm=True, next_weight=w)
+        assert out.shape == shape and h.shape == shape
+        (out.sum() + h.sum()).backward()
+        assert x.grad.shape == shape and w.grad.eq(0).all() and gate.grad.eq(0).all()
+
+
+def test_norm_dtype_rules(device):
+    x = torch.randn(2, 3, 32, device=device)
+    assert nn.rms_norm_modulate(x).dtype == FP32 and nn.rms_norm_modulate(x, dtype=BF16).dtype == BF16
+    assert nn.rms_norm_modulate(x.bfloat16()).dtype == BF16
+    out, h = nn.rms_norm_residual(x, x.half(), next_norm=True)
+    assert out.dtype == FP32 and h.dtype == FP16
+    if device == "cuda":
+        with torch.autocast("cuda", dtype=BF16):
+            assert nn.rms_norm_modulate(x).dtype == BF16 and nn.rms_norm_modulate(x.half()).dtype == FP16
+
+
+def test_norm_refusals(device):
+    x, w = torch.zeros(2, 3, 32, device=device), torch.ones(32, device=device)
+    for bad in (dict(weight=w[:31]), dict(weight=torch.ones(2, 32, device=device)), dict(gate=torch.ones(3, 32, device=device)),
+                dict(gate=torch.ones(2, 3, 32, device=device)), dict(next_weight=w), dict(next_scale=w), dict(eps=0.0),
+                dict(eps=math.nan), dict(residual_scale=math.inf), dict(residual_scale=w)):
+        with pytest.raises(ValueError):
+            nn.rms_norm_residual(x, x, **bad)
+    for bad in (lambda: nn.rms_norm_residual(x, x[:1]), lambda: nn.rms_norm_modulate(torch.zeros(2, 16385, device=device)),
+                lambda: nn.rms_norm_modulate(torch.zeros(2, 0, device=device)),
+                lambda: nn.rms_norm_modulate(torch.zeros((), device=device))):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: nn.rms_norm_residual(x.half(), x), lambda: nn.rms_norm_residual(x.double(), x.double()),
+                lambda: nn.rms_norm_residual(x, x.double()), lambda: nn.rms_norm_residual(x, x, w.double()),
+                lambda: nn.rms_norm_modulate(x.half(), dtype=FP32), lambda: nn.rms_norm_modulate(x, dtype=torch.float64)):
+        with pytest.raises(TypeError):
+            bad()
+
+
+def test_operands_on_two_devices_are_refused():
+    """The meta device stands for another GPU."""
+    x, other = torch.zeros(4, 8), torch.zeros(4, 8, device="meta")
+    plan = nn.plan_experts(torch.zeros(4, 2, dtype=torch.int32), 3)
+    for bad in (lambda: nn.route_tokens(x, 2, bias=other[0]),
+                lambda: nn.route_tokens(x, 2, mask=torch.zeros(4, dtype=torch.bool, device="meta")),
+                lambda: nn.dispatch_tokens(other, plan), lambda: nn.combine_tokens(other.repeat(2, 1), torch.ones(4, 2), plan),
+                lambda: nn.combine_tokens(x.repeat(2, 1), torch.ones(4, 2, device="meta"), plan),
+                lambda: nn.rms_norm_residual(x, other), lambda: nn.rms_norm_modulate(x, other[0])):
+        with pytest.raises(ValueError):
+            bad()

@@ -178,6 +178,72 @@ int vb_gate_residual_backward(const void* dout, int dout_dtype, const void* gate
                               int rows, int cols, int tokens, void* dy, void* dgate, int sums_bf16, float* workspace,
                               long long workspace_floats, unsigned int* tickets, int ticket_count, cudaStream_t stream);
 
+// ---- expert routing (experts.cu) -------------------------------------------------------------------
+// Top-k router over logits [tokens, experts] (dtype: 0 fp32, 1 bf16, 2 fp16; rows `stride` elements apart; experts <= 1024,
+// top_k <= min(experts, 32)).  Keys are fp32(logit) + bias (optional, fp32 [experts]); the top_k largest are chosen, the
+// lowest index first among equals, never a key of -inf.  weights fp32 [tokens, top_k]: softmax over the chosen logits
+// (normalize) or their share of the softmax over all; indices int32, -1 with weight 0 where nothing was left to choose or
+// mask (optional, one byte per token) is 0.  Over the tokens with a choice: counts int32 [experts],
+// balance = experts * sum_e (counts_e / choices) * mean(p_e), z = mean(lse^2); inverse = {1 / tokens, 1 / choices} for the
+// backward call.  workspace: vb_route_workspace floats, any content.
+long long vb_route_workspace(int tokens, int experts);
+int vb_route_forward(const void* logits, int dtype, int tokens, int experts, long long stride, const float* bias,
+                     const uint8_t* mask, int top_k, int normalize, float* weights, int* indices, int* counts,
+                     float* balance, float* z, float* inverse, float* workspace, long long workspace_floats,
+                     cudaStream_t stream);
+// dlogits (contiguous, the logits' dtype) from the optional gradients of weights, balance and z
+int vb_route_backward(const void* logits, int dtype, int tokens, int experts, long long stride, int top_k, int normalize,
+                      const float* weights, const int* indices, const int* counts, const float* inverse,
+                      const float* dweights, const float* dbalance, const float* dz, void* dlogits, cudaStream_t stream);
+// Stable counting sort of n expert choices (int32, or int64 with is_long; values outside [0, experts) are dropped):
+// offsets int32 [experts + 1], the row ranges of the experts; positions int32 [n], the row of every choice or -1.
+long long vb_expert_plan_workspace(int n, int experts);
+int vb_expert_plan(const void* indices, int is_long, int n, int experts, int* offsets, int* positions, int* workspace,
+                   long long workspace_ints, cudaStream_t stream);
+// rows[positions[t, j]] = x[t] byte for byte (rows of an even number of bytes); rows from offsets[experts] on are zeroed.
+// Positions outside [0, tokens * top_k) are skipped, here and below.
+int vb_expert_dispatch(const void* x, long long x_stride_bytes, long long row_bytes, int tokens, int top_k,
+                       const int* positions, const int* offsets, int experts, void* rows, cudaStream_t stream);
+// out[t] = sum_j weights[t, j] * rows[positions[t, j]] (weights null: 1), accumulated in fp32
+int vb_expert_combine(const void* rows, int dtype, int width, int tokens, int top_k, const int* positions,
+                      const void* weights, int weight_dtype, void* out, cudaStream_t stream);
+// drows[positions[t, j]] = weights[t, j] * dout[t] (zero from offsets[experts] on), dweights[t, j] = <dout[t], rows[...]>;
+// drows and dweights may be null
+int vb_expert_combine_backward(const void* dout, const void* rows, int dtype, int width, int tokens, int top_k,
+                               const int* positions, const int* offsets, int experts, const void* weights,
+                               int weight_dtype, void* drows, void* dweights, cudaStream_t stream);
+
+// ---- RMS norms around a block (block_norm.cu) ----------------------------------------------------------
+//   out = residual_scale * x + gate * weight * y * ry,  ry = (mean(y^2) + eps)^-1/2     (with y)
+//   h   = out * ru * next_weight * (1 + next_scale)                                     (with h; out = x without y)
+// x, out: x_dtype; y, h: y_dtype (0 fp32, 1 bf16, 2 fp16; x_dtype is y_dtype or fp32); contiguous [rows, cols],
+// cols <= VB_NORM_MAX_COLS.  A vector is absent (data null), shared (pitch 0) or one row per sample of `tokens` rows.
+#define VB_NORM_MAX_COLS 16384
+typedef struct VbNormVector {
+  const void* data;
+  int dtype;
+  long long pitch;      // elements
+} VbNormVector;
+typedef struct VbBlockNorm {
+  int rows, cols, tokens;
+  int x_dtype, y_dtype;
+  float residual_scale, eps;
+  const void *x, *y;
+  VbNormVector weight, gate, next_weight, next_scale;
+  void *out, *h;
+  float *ry, *ru;       // fp32 [rows]: written by the forward call when not null, read by the backward call
+} VbBlockNorm;
+typedef struct VbBlockNormGrads {
+  const void *dout, *dh;                                      // either may be null
+  void *dx, *dy;                                              // either may be null
+  void *dweight, *dgate, *dnext_weight, *dnext_scale;         // the vectors' dtypes; [cols] or contiguous [samples, cols]; or null
+  float* workspace;                                           // vb_block_norm_workspace floats (any content) when one of the four is asked for
+  long long workspace_floats;
+} VbBlockNormGrads;
+long long vb_block_norm_workspace(int rows, int cols, int tokens);
+int vb_block_norm(const VbBlockNorm* norm, cudaStream_t stream);
+int vb_block_norm_backward(const VbBlockNorm* norm, const VbBlockNormGrads* grads, cudaStream_t stream);
+
 // ---- attention forward for 256-token sequences (tcgen05; one CTA per sample and head) ------------
 // qkv: [batch, 256, 3, heads, head_dim] contiguous (dtype 1 = bf16, 2 = fp16), head_dim a multiple of 8 in [16, 128];
 // out: [batch, 256, heads, head_dim]; lse: [batch, heads, 256] fp32 = log(sum(exp(score * scale))) per query (optional)

@@ -1,0 +1,143 @@
+"""RMS norms before and after a transformer block, fused with the block's gate and the residual scale.
+
+``rms_norm_modulate(x, weight, scale)`` is the norm in front of a block, ``rms_norm_residual(x, y, weight, gate)`` what
+follows it: the block's result ``y`` is normalised, gated and added to the scaled residual stream, and, with
+``next_norm=True``, the new stream is normalised for the next block in the same pass::
+
+    h = rms_norm_modulate(x, w_in, scale_in)
+    x, h = rms_norm_residual(x, block(h), w_out, gate, next_norm=True, next_weight=w_in2, next_scale=scale_in2)
+
+Each call is one kernel forward and one (plus a small one for the gradients of the vectors) backward; nothing but two
+numbers per row is kept besides the inputs.  Vectors are [width] (shared by all rows) or [batch, width] with
+``x`` [batch, ..., width] (one per sample, as an adaLN projection gives them).  CPU tensors take the same path through
+the PyTorch restatement.
+"""
+
+from __future__ import annotations
+
+import math
+from numbers import Real
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def _vector(v, x, name, samples=True):
+    """Check an optional vector; returns whether it has one row per sample."""
+    if v is None:
+        return False
+    if v.dtype not in _DTYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {v.dtype}")
+    if v.device != x.device:
+        raise ValueError(f"{name} is on {v.device}, not on {x.device}")
+    width = x.shape[-1]
+    if v.shape == (width,):
+        return False
+    if samples and x.dim() >= 2 and v.shape == (x.shape[0], width):
+        return True
+    shapes = f"({width},) or (batch, {width})" if samples else f"({width},)"
+    raise ValueError(f"{name} must have shape {shapes} for x of shape {tuple(x.shape)}, got {tuple(v.shape)}")
+
+
+def _in_place(v):
+    """``v`` with unit column stride and rows that do not overlap, as the kernels read it (a copy only if it has not)."""
+    if v is None or ((v.stride(-1) == 1 or v.shape[-1] == 1) and (v.dim() == 1 or v.shape[0] == 1 or v.stride(0) >= v.shape[1])):
+        return v
+    return v.contiguous()
+
+
+class _BlockNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
+        width = x.shape[-1]
+        x2 = x.reshape(-1, width).contiguous()
+        y2 = y.reshape(-1, width).contiguous() if y is not None else None
+        vectors = tuple(_in_place(v) for v in (weight, gate, next_weight, next_scale))
+        out, h, ry, ru = ops.block_norm(x2, y2, *vectors, tokens, residual_scale=residual_scale, eps=eps, h_dtype=h_dtype)
+        ctx.save_for_backward(x2, y2, *vectors, ry, ru)
+        ctx.shape, ctx.tokens, ctx.residual_scale, ctx.eps = x.shape, tokens, residual_scale, eps
+        ctx.set_materialize_grads(False)
+        return out.view(x.shape) if out is not None else None, h.view(x.shape) if h is not None else None
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dh):
+        if dout is None and dh is None:
+            return (None,) * 10
+        x2, y2, *vectors, ry, ru = ctx.saved_tensors
+        dout = dout.reshape(x2.shape).contiguous() if dout is not None else None
+        dh = dh.reshape(x2.shape).contiguous() if dh is not None else None
+        dx, dy, *rest = ops.block_norm_backward(x2, y2, *vectors, ctx.tokens, ry, ru, dout, dh,
+                                                residual_scale=ctx.residual_scale, eps=ctx.eps,
+                                                needs=ctx.needs_input_grad[:6])
+        return (dx.view(ctx.shape) if dx is not None else None, dy.view(ctx.shape) if dy is not None else None, *rest,
+                None, None, None, None)
+
+
+def _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype):
+    width = x.shape[-1] if x.dim() else 0
+    if not 1 <= width <= ops.MAX_NORM_WIDTH:
+        raise ValueError(f"the width must be between 1 and {ops.MAX_NORM_WIDTH}, got x of shape {tuple(x.shape)}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if not (isinstance(eps, Real) and eps > 0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be a positive number, got {eps}")
+    _vector(weight, x, "weight", samples=False)
+    _vector(next_weight, x, "weight" if y is None else "next_weight", samples=False)
+    per_sample = _vector(gate, x, "gate")
+    per_sample |= _vector(next_scale, x, "scale" if y is None else "next_scale")
+    rows = x.numel() // width
+    inputs = (x, y, weight, gate, next_weight, next_scale)
+    if rows == 0:
+        # nothing to compute, but the graph reaches every input
+        empty = sum(t.sum() * 0 for t in inputs if t is not None and t.requires_grad)
+        out = x + empty if y is not None else None
+        return out, (x + empty).to(h_dtype) if h_dtype is not None else None
+    tokens = rows // x.shape[0] if per_sample else rows
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        return _BlockNorm.apply(*inputs, tokens, float(residual_scale), float(eps), h_dtype)
+    x2 = x.detach().reshape(-1, width).contiguous()
+    y2 = y.detach().reshape(-1, width).contiguous() if y is not None else None
+    out, h, _, _ = ops.block_norm(x2, y2, *(_in_place(v) for v in inputs[2:]), tokens, residual_scale=float(residual_scale),
+                                  eps=float(eps), h_dtype=h_dtype, save=False)
+    return out.view(x.shape) if out is not None else None, h.view(x.shape) if h is not None else None
+
+
+def rms_norm_modulate(x, weight=None, scale=None, *, eps=1e-6, dtype=None):
+    """``x * (mean(x^2) + eps)^-1/2 * weight * (1 + scale)`` over the last dimension of ``x`` (at most 16384 wide).
+
+    ``weight`` [width]; ``scale`` [width] or [batch, width].  The result has ``dtype`` (default: the autocast dtype where
+    autocast is on and ``x`` is fp32, else ``x.dtype``); a 16-bit ``x`` keeps its dtype."""
+    if dtype is None:
+        dtype = x.dtype
+        if x.is_cuda and x.dtype == torch.float32 and torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+    if dtype not in _DTYPES or (x.dtype != torch.float32 and dtype != x.dtype):
+        raise TypeError(f"cannot normalise {x.dtype} into {dtype}")
+    return _call(x, None, None, None, weight, scale, 1.0, eps, dtype)[1]
+
+
+def rms_norm_residual(x, y, weight=None, gate=None, *, residual_scale=1.0, eps=1e-6, next_norm=False, next_weight=None,
+                      next_scale=None):
+    """``residual_scale * x + gate * weight * y * (mean(y^2) + eps)^-1/2``: the norm after a block with its gate and the
+    scaled residual connection.  ``x`` is fp32 or has the dtype of ``y``; the result has the dtype of ``x``.
+
+    ``weight`` [width]; ``gate`` [width] or [batch, width].  With ``next_norm`` the result is ``(out, h)`` with
+    ``h = out * (mean(out^2) + eps)^-1/2 * next_weight * (1 + next_scale)`` in the dtype of ``y``, taken from ``out`` before
+    it is rounded: the input of the next block."""
+    if y.shape != x.shape:
+        raise ValueError(f"y must have the shape of x, got {tuple(y.shape)} and {tuple(x.shape)}")
+    if y.dtype not in _DTYPES or x.dtype not in (torch.float32, y.dtype):
+        raise TypeError(f"x must be float32 or have the dtype of y, got {x.dtype} and {y.dtype}")
+    if y.device != x.device:
+        raise ValueError(f"y is on {y.device}, not on {x.device}")
+    if not (isinstance(residual_scale, Real) and math.isfinite(residual_scale)):
+        raise ValueError(f"residual_scale must be a finite number, got {residual_scale}")
+    if not next_norm and (next_weight is not None or next_scale is not None):
+        raise ValueError("next_weight and next_scale need next_norm=True")
+    out, h = _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, y.dtype if next_norm else None)
+    return (out, h) if next_norm else out
