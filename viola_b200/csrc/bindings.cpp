@@ -608,239 +608,6 @@ void gate_residual_backward(const Tensor& dout, const Tensor& gate, const Tensor
         "gate_residual_backward");
 }
 
-// ---- expert routing --------------------------------------------------------------------------------
-static void cuda_typed(const Tensor& t, at::ScalarType type, int64_t numel, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.is_contiguous() && t.scalar_type() == type && t.numel() >= numel, "viola_b200: ", name,
-              " must be a contiguous CUDA tensor of ", type, " with at least ", numel, " elements");
-}
-static int narrow_int(int64_t v, const char* name) {
-  TORCH_CHECK(v >= 0 && v <= INT32_MAX, "viola_b200: ", name, " out of range: ", v);
-  return (int)v;
-}
-
-int64_t route_workspace(int64_t tokens, int64_t experts) {
-  return vb_route_workspace(narrow_int(tokens, "tokens"), narrow_int(experts, "experts"));
-}
-
-void route_forward(const Tensor& logits, const OptTensor& bias, const OptTensor& mask, int64_t top_k, bool normalize,
-                   Tensor weights, Tensor indices, Tensor counts, Tensor balance, Tensor z, Tensor inverse, Tensor workspace) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "logits must be [tokens, experts] with unit stride");
-  const int tokens = narrow_int(logits.size(0), "tokens"), experts = narrow_int(logits.size(1), "experts");
-  if (bias.has_value()) cuda_typed(*bias, at::kFloat, experts, "bias");
-  if (mask.has_value()) cuda_typed(*mask, at::kBool, tokens, "mask");
-  cuda_typed(weights, at::kFloat, tokens * top_k, "weights");
-  cuda_typed(indices, at::kInt, tokens * top_k, "indices");
-  cuda_typed(counts, at::kInt, experts, "counts");
-  cuda_typed(balance, at::kFloat, 1, "balance");
-  cuda_typed(z, at::kFloat, 1, "z");
-  cuda_typed(inverse, at::kFloat, 2, "inverse");
-  cuda_typed(workspace, at::kFloat, 0, "workspace");
-  c10::cuda::CUDAGuard guard(logits.device());
-  check(vb_route_forward(logits.data_ptr(), dtype_code(logits), tokens, experts, logits.stride(0), (const float*)ptr(bias),
-                         (const uint8_t*)ptr(mask), (int)top_k, normalize, weights.data_ptr<float>(), indices.data_ptr<int>(),
-                         counts.data_ptr<int>(), balance.data_ptr<float>(), z.data_ptr<float>(), inverse.data_ptr<float>(),
-                         workspace.data_ptr<float>(), workspace.numel(), stream()),
-        "route_forward");
-}
-
-void route_backward(const Tensor& logits, int64_t top_k, bool normalize, const Tensor& weights, const Tensor& indices,
-                    const Tensor& counts, const Tensor& inverse, const OptTensor& dweights, const OptTensor& dbalance,
-                    const OptTensor& dz, Tensor dlogits) {
-  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.stride(1) == 1, "logits must be [tokens, experts] with unit stride");
-  const int tokens = narrow_int(logits.size(0), "tokens"), experts = narrow_int(logits.size(1), "experts");
-  cuda_typed(weights, at::kFloat, tokens * top_k, "weights");
-  cuda_typed(indices, at::kInt, tokens * top_k, "indices");
-  cuda_typed(counts, at::kInt, experts, "counts");
-  cuda_typed(inverse, at::kFloat, 2, "inverse");
-  if (dweights.has_value()) cuda_typed(*dweights, at::kFloat, tokens * top_k, "dweights");
-  if (dbalance.has_value()) cuda_typed(*dbalance, at::kFloat, 1, "dbalance");
-  if (dz.has_value()) cuda_typed(*dz, at::kFloat, 1, "dz");
-  cuda_typed(dlogits, logits.scalar_type(), logits.numel(), "dlogits");
-  c10::cuda::CUDAGuard guard(logits.device());
-  check(vb_route_backward(logits.data_ptr(), dtype_code(logits), tokens, experts, logits.stride(0), (int)top_k, normalize,
-                          weights.data_ptr<float>(), indices.data_ptr<int>(), counts.data_ptr<int>(),
-                          inverse.data_ptr<float>(), (const float*)ptr(dweights), (const float*)ptr(dbalance),
-                          (const float*)ptr(dz), dlogits.data_ptr(), stream()),
-        "route_backward");
-}
-
-int64_t expert_plan_workspace(int64_t choices, int64_t experts) {
-  return vb_expert_plan_workspace(narrow_int(choices, "choices"), narrow_int(experts, "experts"));
-}
-
-void expert_plan(const Tensor& indices, int64_t experts, Tensor offsets, Tensor positions, const OptTensor& workspace) {
-  cuda_contig(indices, "indices");
-  TORCH_CHECK(indices.scalar_type() == at::kInt || indices.scalar_type() == at::kLong, "indices must be int32 or int64");
-  const int n = narrow_int(indices.numel(), "choices");
-  cuda_typed(offsets, at::kInt, experts + 1, "offsets");
-  cuda_typed(positions, at::kInt, n, "positions");
-  if (workspace.has_value()) cuda_typed(*workspace, at::kInt, 0, "workspace");
-  c10::cuda::CUDAGuard guard(indices.device());
-  check(vb_expert_plan(indices.data_ptr(), indices.scalar_type() == at::kLong, n, narrow_int(experts, "experts"),
-                       offsets.data_ptr<int>(), positions.data_ptr<int>(), (int*)ptr(workspace),
-                       workspace.has_value() ? workspace->numel() : 0, stream()),
-        "expert_plan");
-}
-
-// positions [tokens, top_k] and offsets [experts + 1] of a plan
-static void check_plan(const Tensor& positions, const Tensor& offsets) {
-  TORCH_CHECK(positions.dim() == 2 && offsets.dim() == 1 && offsets.numel() >= 2);
-  cuda_typed(positions, at::kInt, 0, "positions");
-  cuda_typed(offsets, at::kInt, 2, "offsets");
-}
-
-void expert_dispatch(const Tensor& x, const Tensor& positions, const Tensor& offsets, Tensor rows) {
-  check_plan(positions, offsets);
-  cuda_contig(rows, "rows");
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.stride(1) == 1 && x.size(0) == positions.size(0), "x must be [tokens, width]");
-  TORCH_CHECK(rows.dim() == 2 && rows.scalar_type() == x.scalar_type() && rows.size(0) == positions.numel() &&
-              rows.size(1) == x.size(1));
-  c10::cuda::CUDAGuard guard(x.device());
-  check(vb_expert_dispatch(x.data_ptr(), x.stride(0) * x.element_size(), x.size(1) * x.element_size(),
-                           narrow_int(x.size(0), "tokens"), (int)positions.size(1), positions.data_ptr<int>(),
-                           offsets.data_ptr<int>(), (int)offsets.numel() - 1, rows.data_ptr(), stream()),
-        "expert_dispatch");
-}
-
-void expert_combine(const Tensor& rows, const Tensor& positions, const OptTensor& weights, Tensor out) {
-  cuda_typed(positions, at::kInt, 0, "positions");
-  cuda_contig(rows, "rows");
-  cuda_contig(out, "out");
-  TORCH_CHECK(positions.dim() == 2 && rows.dim() == 2 && out.dim() == 2 && rows.size(0) == positions.numel() &&
-              out.size(0) == positions.size(0) && out.size(1) == rows.size(1) && out.scalar_type() == rows.scalar_type());
-  if (weights.has_value()) {
-    cuda_contig(*weights, "weights");
-    TORCH_CHECK(weights->numel() == positions.numel());
-  }
-  c10::cuda::CUDAGuard guard(rows.device());
-  check(vb_expert_combine(rows.data_ptr(), dtype_code(rows), narrow_int(rows.size(1), "width"),
-                          narrow_int(positions.size(0), "tokens"), (int)positions.size(1), positions.data_ptr<int>(),
-                          ptr(weights), weights.has_value() ? dtype_code(*weights) : 0, out.data_ptr(), stream()),
-        "expert_combine");
-}
-
-void expert_combine_backward(const Tensor& dout, const Tensor& rows, const Tensor& positions, const Tensor& offsets,
-                             const Tensor& weights, const OptTensor& drows, const OptTensor& dweights) {
-  check_plan(positions, offsets);
-  cuda_contig(dout, "dout");
-  cuda_contig(rows, "rows");
-  cuda_contig(weights, "weights");
-  TORCH_CHECK(rows.dim() == 2 && dout.dim() == 2 && rows.size(0) == positions.numel() && dout.size(0) == positions.size(0) &&
-              dout.size(1) == rows.size(1) && dout.scalar_type() == rows.scalar_type() && weights.numel() == positions.numel());
-  if (drows.has_value()) cuda_typed(*drows, rows.scalar_type(), rows.numel(), "drows");
-  if (dweights.has_value()) cuda_typed(*dweights, weights.scalar_type(), weights.numel(), "dweights");
-  c10::cuda::CUDAGuard guard(rows.device());
-  check(vb_expert_combine_backward(dout.data_ptr(), rows.data_ptr(), dtype_code(rows), narrow_int(rows.size(1), "width"),
-                                   narrow_int(positions.size(0), "tokens"), (int)positions.size(1), positions.data_ptr<int>(),
-                                   offsets.data_ptr<int>(), (int)offsets.numel() - 1, weights.data_ptr(), dtype_code(weights),
-                                   ptr(drows), ptr(dweights), stream()),
-        "expert_combine_backward");
-}
-
-// ---- RMS norms around a block ------------------------------------------------------------------------
-// [cols]: shared; [samples, cols] with unit column stride: one row per sample
-static VbNormVector norm_vector(const OptTensor& t, int64_t samples, int64_t cols, const char* name) {
-  if (!t.has_value()) return VbNormVector{nullptr, 0, 0};
-  TORCH_CHECK(t->is_cuda() && (t->dim() == 1 || t->dim() == 2) && t->size(-1) == cols && (cols == 1 || t->stride(-1) == 1), name,
-              " must be a CUDA vector of the row width, or one per sample, with unit column stride");
-  if (t->dim() == 1) return VbNormVector{t->data_ptr(), dtype_code(*t), 0};
-  TORCH_CHECK(t->size(0) == samples && (samples == 1 || t->stride(0) >= cols), name, " must have one row per sample");
-  return VbNormVector{t->data_ptr(), dtype_code(*t), samples == 1 ? cols : t->stride(0)};
-}
-
-static VbBlockNorm block_norm_args(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate,
-                                   const OptTensor& next_weight, const OptTensor& next_scale, int64_t tokens,
-                                   double residual_scale, double eps) {
-  cuda_contig(x, "x");
-  TORCH_CHECK(x.dim() == 2 && tokens >= 1 && x.size(0) % tokens == 0);
-  VbBlockNorm n{};
-  n.rows = narrow_int(x.size(0), "rows");
-  n.cols = narrow_int(x.size(1), "cols");
-  n.tokens = narrow_int(tokens, "tokens");
-  n.x_dtype = dtype_code(x);
-  n.residual_scale = (float)residual_scale;
-  n.eps = (float)eps;
-  n.x = x.data_ptr();
-  if (y.has_value()) {
-    cuda_contig(*y, "y");
-    TORCH_CHECK(y->sizes() == x.sizes());
-    n.y = y->data_ptr();
-  }
-  const int64_t samples = x.size(0) / tokens;
-  n.weight = norm_vector(weight, samples, x.size(1), "weight");
-  n.gate = norm_vector(gate, samples, x.size(1), "gate");
-  n.next_weight = norm_vector(next_weight, samples, x.size(1), "next_weight");
-  n.next_scale = norm_vector(next_scale, samples, x.size(1), "next_scale");
-  return n;
-}
-static void* like(const OptTensor& t, const Tensor& x, const char* name) {
-  if (!t.has_value()) return nullptr;
-  cuda_contig(*t, name);
-  TORCH_CHECK(t->sizes() == x.sizes(), name, " must have the shape of x");
-  return t->data_ptr();
-}
-static float* row_values(const OptTensor& t, const Tensor& x, const char* name) {
-  if (!t.has_value()) return nullptr;
-  cuda_typed(*t, at::kFloat, x.size(0), name);
-  return t->data_ptr<float>();
-}
-
-int64_t block_norm_workspace(int64_t rows, int64_t cols, int64_t tokens) {
-  return vb_block_norm_workspace(narrow_int(rows, "rows"), narrow_int(cols, "cols"), narrow_int(tokens, "tokens"));
-}
-
-void block_norm(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate,
-                const OptTensor& next_weight, const OptTensor& next_scale, int64_t tokens, double residual_scale, double eps,
-                const OptTensor& out, const OptTensor& h, const OptTensor& ry, const OptTensor& ru) {
-  VbBlockNorm n = block_norm_args(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps);
-  n.out = like(out, x, "out");
-  n.h = like(h, x, "h");
-  TORCH_CHECK(!out.has_value() || out->scalar_type() == x.scalar_type());
-  TORCH_CHECK(!y.has_value() || !h.has_value() || y->scalar_type() == h->scalar_type());
-  n.y_dtype = y.has_value() ? dtype_code(*y) : h.has_value() ? dtype_code(*h) : n.x_dtype;
-  n.ry = row_values(ry, x, "ry");
-  n.ru = row_values(ru, x, "ru");
-  c10::cuda::CUDAGuard guard(x.device());
-  check(vb_block_norm(&n, stream()), "block_norm");
-}
-
-void block_norm_backward(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate,
-                         const OptTensor& next_weight, const OptTensor& next_scale, int64_t tokens, double residual_scale,
-                         double eps, const OptTensor& ry, const OptTensor& ru, const OptTensor& dout, const OptTensor& dh,
-                         const OptTensor& dx, const OptTensor& dy, const OptTensor& dweight, const OptTensor& dgate,
-                         const OptTensor& dnext_weight, const OptTensor& dnext_scale, const OptTensor& workspace) {
-  VbBlockNorm n = block_norm_args(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps);
-  n.ry = row_values(ry, x, "ry");
-  n.ru = row_values(ru, x, "ru");
-  n.y_dtype = y.has_value() ? dtype_code(*y) : dh.has_value() ? dtype_code(*dh) : n.x_dtype;
-  TORCH_CHECK(!dh.has_value() || dtype_code(*dh) == n.y_dtype, "dh must have the dtype of y");
-  TORCH_CHECK(!dout.has_value() || dtype_code(*dout) == n.x_dtype, "dout must have the dtype of x");
-  TORCH_CHECK(!dx.has_value() || dtype_code(*dx) == n.x_dtype, "dx must have the dtype of x");
-  TORCH_CHECK(!dy.has_value() || dtype_code(*dy) == n.y_dtype, "dy must have the dtype of y");
-  VbBlockNormGrads g{};
-  g.dout = like(dout, x, "dout");
-  g.dh = like(dh, x, "dh");
-  g.dx = like(dx, x, "dx");
-  g.dy = like(dy, x, "dy");
-  auto vector_grad = [](const OptTensor& grad, const OptTensor& vector, const char* name) -> void* {
-    if (!grad.has_value()) return nullptr;
-    TORCH_CHECK(vector.has_value() && grad->is_cuda() && grad->is_contiguous() && grad->sizes() == vector->sizes() &&
-                grad->scalar_type() == vector->scalar_type(), name, " must look like its vector, contiguous");
-    return grad->data_ptr();
-  };
-  g.dweight = vector_grad(dweight, weight, "dweight");
-  g.dgate = vector_grad(dgate, gate, "dgate");
-  g.dnext_weight = vector_grad(dnext_weight, next_weight, "dnext_weight");
-  g.dnext_scale = vector_grad(dnext_scale, next_scale, "dnext_scale");
-  if (workspace.has_value()) {
-    cuda_typed(*workspace, at::kFloat, 0, "workspace");
-    g.workspace = workspace->data_ptr<float>();
-    g.workspace_floats = workspace->numel();
-  }
-  c10::cuda::CUDAGuard guard(x.device());
-  check(vb_block_norm_backward(&n, &g, stream()), "block_norm_backward");
-}
-
 // ---- multi-tensor optimizer kernels ---------------------------------------------------------------
 void multi_ema(const Tensor& table, const Tensor& prefix, int64_t blocks, double decay) {
   c10::cuda::CUDAGuard guard(table.device());
@@ -917,17 +684,6 @@ TORCH_LIBRARY(viola_b200, m) {
   m.def("fused_quantize", &fused_quantize);
   m.def("ln_modulate_backward", &ln_modulate_backward);
   m.def("row_block_count", &row_block_count);
-  m.def("route_workspace", &route_workspace);
-  m.def("route_forward", &route_forward);
-  m.def("route_backward", &route_backward);
-  m.def("expert_plan_workspace", &expert_plan_workspace);
-  m.def("expert_plan", &expert_plan);
-  m.def("expert_dispatch", &expert_dispatch);
-  m.def("expert_combine", &expert_combine);
-  m.def("expert_combine_backward", &expert_combine_backward);
-  m.def("block_norm_workspace", &block_norm_workspace);
-  m.def("block_norm", &block_norm);
-  m.def("block_norm_backward", &block_norm_backward);
   m.def("gate_residual", &gate_residual);
   m.def("gate_residual_backward", &gate_residual_backward);
 }

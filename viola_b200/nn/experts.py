@@ -18,7 +18,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -52,34 +51,6 @@ def _same_device(tensor, name, other):
         raise ValueError(f"{name} is on {tensor.device}, not on {other.device}")
 
 
-def _rows2d(x):
-    x = x.reshape(-1, x.shape[-1])
-    return x if x.stride(1) == 1 or x.shape[1] == 1 and x.is_contiguous() else x.contiguous()
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, bias, mask, top_k, normalize):
-        flat = _rows2d(logits)
-        weights, indices, counts, balance, z, inverse = ops.route_forward(
-            flat, top_k, bias=bias, mask=mask, normalize=normalize, lead=logits.shape[:-1])
-        ctx.save_for_backward(flat, weights, indices, counts, inverse)
-        ctx.top_k, ctx.normalize, ctx.shape = top_k, normalize, logits.shape
-        ctx.mark_non_differentiable(indices, counts)
-        ctx.set_materialize_grads(False)
-        return weights, indices, counts, balance, z
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dweights, _dindices, _dcounts, dbalance, dz):
-        if dweights is None and dbalance is None and dz is None:
-            return (None,) * 5
-        flat, weights, indices, counts, inverse = ctx.saved_tensors
-        dlogits = ops.route_backward(flat, ctx.top_k, weights, indices, counts, inverse, normalize=ctx.normalize,
-                                     dweights=None if dweights is None else dweights.contiguous(), dbalance=dbalance, dz=dz)
-        return dlogits.view(ctx.shape), None, None, None, None
-
-
 def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
     """Chooses ``top_k`` experts for every token of ``logits`` [..., experts] (up to 1024 experts, ``top_k`` up to 32).
 
@@ -108,11 +79,8 @@ def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
         if mask.dtype != torch.bool or mask.shape != logits.shape[:-1]:
             raise ValueError(f"mask must be bool of shape {tuple(logits.shape[:-1])}, got {mask.dtype} {tuple(mask.shape)}")
         _same_device(mask, "mask", logits)
-        mask = mask.reshape(-1).contiguous()
-    if logits.requires_grad and torch.is_grad_enabled():
-        return Routing(*_Route.apply(logits, bias, mask, top_k, normalize))
-    return Routing(*ops.route_forward(_rows2d(logits.detach()), top_k, bias=bias, mask=mask, normalize=normalize,
-                                      lead=logits.shape[:-1])[:5])
+        mask = mask.contiguous()
+    return Routing(*ops.route(logits, top_k, bias=bias, mask=mask, normalize=normalize))
 
 
 def plan_experts(indices, num_experts):
@@ -124,7 +92,7 @@ def plan_experts(indices, num_experts):
         raise ValueError(f"the number of experts must be between 1 and {ops.MAX_EXPERTS}, got {num_experts}")
     if not 1 <= indices.shape[-1] <= ops.MAX_TOP_K:
         raise ValueError(f"indices must hold between 1 and {ops.MAX_TOP_K} choices per token, got {indices.shape[-1]}")
-    return ExpertPlan(*ops.expert_plan(indices.reshape(-1, indices.shape[-1]), num_experts))
+    return ExpertPlan(*ops.expert_plan(indices, num_experts))
 
 
 def _check_plan(plan, tensor, name):
@@ -139,20 +107,6 @@ def _check_plan(plan, tensor, name):
     return offsets.contiguous(), positions.contiguous()
 
 
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, positions, offsets):
-        ctx.save_for_backward(positions)
-        ctx.shape = x.shape
-        return ops.expert_dispatch(_rows2d(x), positions, offsets)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, drows):
-        positions, = ctx.saved_tensors
-        return ops.expert_combine(drows.contiguous(), positions).view(ctx.shape), None, None
-
-
 def dispatch_tokens(x, plan):
     """The rows of ``x`` [..., width] sorted by expert: [tokens * top_k, width], one row per choice, zeros behind the last
     expert's rows (``plan.offsets[-1]``)."""
@@ -161,26 +115,7 @@ def dispatch_tokens(x, plan):
     width = x.shape[-1]
     if width < 1 or x.numel() != positions.shape[0] * width:
         raise ValueError(f"x of shape {tuple(x.shape)} does not hold the plan's {positions.shape[0]} tokens")
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Dispatch.apply(x, positions, offsets)
-    return ops.expert_dispatch(_rows2d(x.detach()), positions, offsets)
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, weights, positions, offsets):
-        rows, flat = rows.contiguous(), weights.contiguous()
-        ctx.save_for_backward(rows, flat, positions, offsets)
-        return ops.expert_combine(rows, positions, flat).view(*weights.shape[:-1], rows.shape[1])
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout):
-        rows, weights, positions, offsets = ctx.saved_tensors
-        drows, dweights = ops.expert_combine_backward(
-            dout.reshape(-1, rows.shape[1]).contiguous(), rows, positions, offsets, weights,
-            need_rows=ctx.needs_input_grad[0], need_weights=ctx.needs_input_grad[1])
-        return drows, dweights, None, None
+    return ops.expert_dispatch(x, positions, offsets)
 
 
 def combine_tokens(rows, weights, plan):
@@ -198,7 +133,4 @@ def combine_tokens(rows, weights, plan):
         raise ValueError(f"rows must be [{tokens * top_k}, width], got {tuple(rows.shape)}")
     if weights.dim() < 1 or weights.shape[-1] != top_k or weights.numel() != tokens * top_k:
         raise ValueError(f"weights of shape {tuple(weights.shape)} do not match the plan's {tokens} tokens x {top_k} choices")
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
-        return _Combine.apply(rows, weights, positions, offsets)
-    return ops.expert_combine(rows.detach().contiguous(), positions, weights.detach().contiguous()).view(
-        *weights.shape[:-1], rows.shape[1])
+    return ops.expert_combine(rows, weights, positions, offsets)

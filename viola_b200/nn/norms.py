@@ -19,7 +19,6 @@ import math
 from numbers import Real
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -43,41 +42,6 @@ def _vector(v, x, name, samples=True):
     raise ValueError(f"{name} must have shape {shapes} for x of shape {tuple(x.shape)}, got {tuple(v.shape)}")
 
 
-def _in_place(v):
-    """``v`` with unit column stride and rows that do not overlap, as the kernels read it (a copy only if it has not)."""
-    if v is None or ((v.stride(-1) == 1 or v.shape[-1] == 1) and (v.dim() == 1 or v.shape[0] == 1 or v.stride(0) >= v.shape[1])):
-        return v
-    return v.contiguous()
-
-
-class _BlockNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
-        width = x.shape[-1]
-        x2 = x.reshape(-1, width).contiguous()
-        y2 = y.reshape(-1, width).contiguous() if y is not None else None
-        vectors = tuple(_in_place(v) for v in (weight, gate, next_weight, next_scale))
-        out, h, ry, ru = ops.block_norm(x2, y2, *vectors, tokens, residual_scale=residual_scale, eps=eps, h_dtype=h_dtype)
-        ctx.save_for_backward(x2, y2, *vectors, ry, ru)
-        ctx.shape, ctx.tokens, ctx.residual_scale, ctx.eps = x.shape, tokens, residual_scale, eps
-        ctx.set_materialize_grads(False)
-        return out.view(x.shape) if out is not None else None, h.view(x.shape) if h is not None else None
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dh):
-        if dout is None and dh is None:
-            return (None,) * 10
-        x2, y2, *vectors, ry, ru = ctx.saved_tensors
-        dout = dout.reshape(x2.shape).contiguous() if dout is not None else None
-        dh = dh.reshape(x2.shape).contiguous() if dh is not None else None
-        dx, dy, *rest = ops.block_norm_backward(x2, y2, *vectors, ctx.tokens, ry, ru, dout, dh,
-                                                residual_scale=ctx.residual_scale, eps=ctx.eps,
-                                                needs=ctx.needs_input_grad[:6])
-        return (dx.view(ctx.shape) if dx is not None else None, dy.view(ctx.shape) if dy is not None else None, *rest,
-                None, None, None, None)
-
-
 def _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype):
     width = x.shape[-1] if x.dim() else 0
     if not 1 <= width <= ops.MAX_NORM_WIDTH:
@@ -98,13 +62,8 @@ def _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dt
         out = x + empty if y is not None else None
         return out, (x + empty).to(h_dtype) if h_dtype is not None else None
     tokens = rows // x.shape[0] if per_sample else rows
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
-        return _BlockNorm.apply(*inputs, tokens, float(residual_scale), float(eps), h_dtype)
-    x2 = x.detach().reshape(-1, width).contiguous()
-    y2 = y.detach().reshape(-1, width).contiguous() if y is not None else None
-    out, h, _, _ = ops.block_norm(x2, y2, *(_in_place(v) for v in inputs[2:]), tokens, residual_scale=float(residual_scale),
-                                  eps=float(eps), h_dtype=h_dtype, save=False)
-    return out.view(x.shape) if out is not None else None, h.view(x.shape) if h is not None else None
+    results = ops.block_norm(*inputs, tokens, float(residual_scale), float(eps), h_dtype)
+    return results[0] if y is not None else None, results[-1] if h_dtype is not None else None
 
 
 def rms_norm_modulate(x, weight=None, scale=None, *, eps=1e-6, dtype=None):

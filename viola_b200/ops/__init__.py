@@ -10,7 +10,6 @@ reads the same.
 
 from __future__ import annotations
 
-import functools
 import math
 import os
 import threading
@@ -885,153 +884,59 @@ def gate_residual_backward(dout, gate, y, tokens, sums_dtype=torch.float32):
 
 
 # ------------------------------------------------------------------------------ expert routing
+# These operators and the norms below allocate their results and record their gradients in C++ (csrc/functions.cpp);
+# :func:`block_launches` counts the kernels launched there.  On the CPU autograd differentiates the restatements.
 MAX_EXPERTS, MAX_TOP_K = 1024, 32
 
 
-@functools.lru_cache(maxsize=1024)
-def _route_workspace(tokens, experts):
-    return _ops().route_workspace(tokens, experts)
+def block_launches():
+    """Kernels launched so far by the operators that record their own gradients."""
+    return _ops().block_launches()
 
 
-@functools.lru_cache(maxsize=1024)
-def _plan_workspace(choices, experts):
-    return _ops().expert_plan_workspace(choices, experts)
-
-
-def route_forward(logits, top_k, *, bias=None, mask=None, normalize=True, lead=None):
-    """Top-k router over ``logits`` [tokens, experts]: (weights fp32, indices int32 [tokens, top_k], counts int32
-    [experts], balance, z, inverse).  ``bias`` fp32 [experts] is added to the logits for the choice alone; tokens whose
-    ``mask`` is False, or that have no logit above -inf, get index -1 and weight 0 and enter no sum.  ``inverse`` holds
-    the reciprocals of the numbers of counted tokens and choices for :func:`route_backward`.  ``lead``: leading shape of
-    the per-token results (default ``(tokens,)``)."""
-    tokens, experts = logits.shape
-    lead = (tokens,) if lead is None else tuple(lead)
+def route(logits, top_k, *, bias=None, mask=None, normalize=True):
+    """Top-k router over ``logits`` [..., experts]: (weights fp32, indices int32 [..., top_k], counts int32 [experts],
+    balance, z).  ``bias`` (fp32 [experts]) is added to the logits for the choice alone; tokens whose ``mask`` is False, or
+    that have no key above -inf, get index -1 and weight 0 and enter no sum."""
     if not logits.is_cuda:
-        weights, indices, *rest = reference.route_forward(logits, top_k, bias=bias, mask=mask, normalize=normalize)
-        return (weights.view(*lead, top_k), indices.view(*lead, top_k), *rest)
-    device = logits.device
-    weights = torch.empty((*lead, top_k), device=device, dtype=torch.float32)
-    indices = torch.empty((*lead, top_k), device=device, dtype=torch.int32)
-    counts = torch.empty(experts, device=device, dtype=torch.int32)
-    balance, z = torch.empty((), device=device, dtype=torch.float32), torch.empty((), device=device, dtype=torch.float32)
-    inverse = torch.empty(2, device=device, dtype=torch.float32)
-    # a workspace of this call's own: two captured graphs, or two streams, never share one
-    workspace = torch.empty(_route_workspace(tokens, experts), device=device, dtype=torch.float32)
-    _ops().route_forward(logits, bias, mask, top_k, normalize, weights, indices, counts, balance, z, inverse, workspace)
-    _count()
-    return weights, indices, counts, balance, z, inverse
-
-
-def route_backward(logits, top_k, weights, indices, counts, inverse, *, normalize=True, dweights=None, dbalance=None,
-                   dz=None):
-    """Gradient of the logits [tokens, experts] from the optional gradients of the weights and the two losses."""
-    if not logits.is_cuda:
-        k = indices.shape[-1]
-        return reference.route_backward(logits, top_k, weights.reshape(-1, k), indices.reshape(-1, k), counts, inverse,
-                                        normalize=normalize, dbalance=dbalance, dz=dz,
-                                        dweights=None if dweights is None else dweights.reshape(-1, k))
-    dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-    _ops().route_backward(logits, top_k, normalize, weights, indices, counts, inverse, dweights, dbalance, dz, dlogits)
-    _count()
-    return dlogits
+        return reference.route(logits, top_k, bias=bias, mask=mask, normalize=normalize)
+    return _ops().route(logits, top_k, bias, mask, normalize)
 
 
 def expert_plan(indices, experts):
-    """Stable counting sort of expert choices [tokens, top_k] (int32 or int64; others than 0 .. experts - 1 are dropped):
+    """Stable counting sort of expert choices [..., top_k] (int32 or int64; others than 0 .. experts - 1 are dropped):
     (offsets int32 [experts + 1], positions int32 [tokens, top_k], -1 for a dropped choice)."""
     if not indices.is_cuda:
         return reference.expert_plan(indices, experts)
-    indices = indices.contiguous()
-    offsets = torch.empty(experts + 1, device=indices.device, dtype=torch.int32)
-    positions = torch.empty(indices.shape, device=indices.device, dtype=torch.int32)
-    need = _plan_workspace(indices.numel(), experts)
-    workspace = torch.empty(need, device=indices.device, dtype=torch.int32) if need else None
-    _ops().expert_plan(indices, experts, offsets, positions, workspace)
-    _count(2 if need else 1)
-    return offsets, positions
+    return _ops().expert_plan(indices, experts)
 
 
 def expert_dispatch(x, positions, offsets):
     """Rows sorted by expert: ``rows[positions[t, j]] = x[t]`` ([tokens * top_k, width]; rows behind the last are zero)."""
     if not x.is_cuda:
         return reference.expert_dispatch(x, positions, offsets)
-    rows = torch.empty((positions.numel(), x.shape[1]), device=x.device, dtype=x.dtype)
-    _ops().expert_dispatch(x, positions, offsets, rows)
-    _count()
-    return rows
+    return _ops().expert_dispatch(x, positions, offsets)
 
 
-def expert_combine(rows, positions, weights=None):
-    """``out[t] = sum_j weights[t, j] * rows[positions[t, j]]`` in fp32, rounded once (``weights`` None: all one, which is
-    the gradient of :func:`expert_dispatch`)."""
+def expert_combine(rows, weights, positions, offsets):
+    """``out[t] = sum_j weights[t, j] * rows[positions[t, j]]`` in fp32, rounded once."""
     if not rows.is_cuda:
-        return reference.expert_combine(rows, positions, weights)
-    out = torch.empty((positions.shape[0], rows.shape[1]), device=rows.device, dtype=rows.dtype)
-    _ops().expert_combine(rows, positions, weights, out)
-    _count()
-    return out
-
-
-def expert_combine_backward(dout, rows, positions, offsets, weights, *, need_rows=True, need_weights=True):
-    """Gradients of :func:`expert_combine`: (drows, dweights), None for one that is not needed."""
-    if not rows.is_cuda:
-        drows, dweights = reference.expert_combine_backward(dout, rows, positions, offsets, weights)
-        return drows if need_rows else None, dweights if need_weights else None
-    drows = torch.empty(rows.shape, device=rows.device, dtype=rows.dtype) if need_rows else None
-    dweights = torch.empty(weights.shape, device=rows.device, dtype=weights.dtype) if need_weights else None
-    _ops().expert_combine_backward(dout, rows, positions, offsets, weights, drows, dweights)
-    _count()
-    return drows, dweights
+        return reference.expert_combine(rows, weights, positions, offsets)
+    return _ops().expert_combine(rows, weights, positions, offsets)
 
 
 # ------------------------------------------------------------------------------ RMS norms around a block
 MAX_NORM_WIDTH = 16384
 
 
-@functools.lru_cache(maxsize=1024)
-def _block_norm_workspace(rows, cols, tokens):
-    return _ops().block_norm_workspace(rows, cols, tokens)
-
-
-def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, *, residual_scale=1.0, eps=1e-6, h_dtype=None,
-               save=True):
+def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
     """``out = residual_scale * x + gate * weight * rms(y)`` (with ``y``) and ``h = rms(out) * next_weight * (1 + next_scale)``
-    (with ``h_dtype``; ``out`` is ``x`` without ``y``) for [rows, cols] tensors; the vectors are [cols] or one row per
-    sample of ``tokens`` rows.  Returns (out, h, ry, ru): the reciprocal roots are for :func:`block_norm_backward`, None
-    unless ``save``."""
+    (with ``h_dtype``; ``out`` is ``x`` without ``y``) over the last dimension; the vectors are [width] or one row per
+    sample of ``tokens`` rows.  Returns those of (out, h) that were asked for."""
     if not x.is_cuda:
-        return reference.block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale=residual_scale,
-                                    eps=eps, h_dtype=h_dtype)
-    out = torch.empty(x.shape, device=x.device, dtype=x.dtype) if y is not None else None
-    h = torch.empty(x.shape, device=x.device, dtype=h_dtype) if h_dtype is not None else None
-    ry = ru = None
-    if save:
-        ry = torch.empty(x.shape[0], device=x.device, dtype=torch.float32) if y is not None else None
-        ru = torch.empty(x.shape[0], device=x.device, dtype=torch.float32) if h_dtype is not None else None
-    _ops().block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, out, h, ry, ru)
-    _count()
-    return out, h, ry, ru
-
-
-def block_norm_backward(x, y, weight, gate, next_weight, next_scale, tokens, ry, ru, dout, dh, *, residual_scale=1.0,
-                        eps=1e-6, needs=(True,) * 6):
-    """Gradients (dx, dy, dweight, dgate, dnext_weight, dnext_scale) from those of ``out`` and ``h`` (either may be None);
-    ``needs`` says which are wanted, the others come back as None."""
-    if not x.is_cuda:
-        grads = reference.block_norm_backward(x, y, weight, gate, next_weight, next_scale, tokens, ry, ru, dout, dh,
-                                              residual_scale=residual_scale)
-        return tuple(g if need else None for g, need in zip(grads, needs))
-    tensors = (x, y if y is not None else None, weight if y is not None else None, gate if y is not None else None,
-               next_weight if dh is not None else None, next_scale if dh is not None else None)
-    grads = [torch.empty(t.shape, device=x.device, dtype=t.dtype) if need and t is not None else None
-             for t, need in zip(tensors, needs)]
-    workspace, sums = None, any(g is not None for g in grads[2:])
-    if sums:
-        workspace = torch.empty(_block_norm_workspace(*x.shape, tokens), device=x.device, dtype=torch.float32)
-    _ops().block_norm_backward(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, ry, ru, dout, dh,
-                               *grads, workspace)
-    _count(2 if sums else 1)
-    return tuple(grads)
+        return reference.block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype)
+    return _ops().block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps,
+                             -1 if h_dtype is None else _DT[h_dtype])
 
 
 # ------------------------------------------------------------------------------ multi-tensor optimizer ops

@@ -481,13 +481,14 @@ def mx_gemm(a, b, sa, sb, *, out_dtype, bias=None):
 
 
 # --------------------------------------------------------------------------- expert routing
-def route_forward(logits, top_k, *, bias=None, mask=None, normalize=True):
-    """Router of :func:`viola_b200.ops.route_forward` on [tokens, experts] logits."""
-    tokens, experts = logits.shape
-    values = logits.float()
+# These and the norms below are written for autograd to differentiate: what a masked place holds (infinities, NaN) is
+# replaced before it enters any arithmetic, and 16-bit values are widened once, so that gradients are summed in fp32.
+def route(logits, top_k, *, bias=None, mask=None, normalize=True):
+    experts, lead = logits.shape[-1], logits.shape[:-1]
+    values = logits.reshape(-1, experts).float()
     if mask is not None:
-        values = torch.where(mask[:, None], values, -math.inf)
-    key = values if bias is None else values + bias.float()
+        values = torch.where(mask.reshape(-1, 1), values, -math.inf)
+    key = values.detach() if bias is None else values.detach() + bias.float()
     ranked, order = key.sort(dim=1, descending=True, stable=True)
     indices = torch.where(ranked[:, :top_k] == -math.inf, -1, order[:, :top_k])
     chosen = indices >= 0
@@ -496,137 +497,65 @@ def route_forward(logits, top_k, *, bias=None, mask=None, normalize=True):
     p, lse = torch.softmax(safe, dim=1), torch.logsumexp(safe, dim=1)
     at = indices.clamp_min(0)
     if normalize:
-        weights = torch.softmax(torch.where(chosen, safe.gather(1, at), -math.inf), dim=1)
+        picked = torch.where(chosen, safe.gather(1, at), -math.inf)
+        weights = torch.softmax(torch.where(live[:, None], picked, 0.0), dim=1)
     else:
         weights = p.gather(1, at)
     weights = torch.where(chosen, weights, 0.0)
     counts = torch.bincount(indices[chosen], minlength=experts).to(torch.int32)
-    inverse = 1.0 / torch.stack([live.sum(), counts.sum()]).clamp_min(1).float()
-    p_sum = torch.where(live[:, None], p, 0.0).sum(0)
-    balance = experts * (counts * p_sum).sum() * inverse[0] * inverse[1]
-    z = torch.where(live, lse * lse, 0.0).sum() * inverse[0]
-    return weights, indices.to(torch.int32), counts, balance, z, inverse
-
-
-def route_backward(logits, top_k, weights, indices, counts, inverse, *, normalize=True, dweights=None, dbalance=None,
-                   dz=None):
-    experts = logits.shape[1]
-    live = indices[:, :1] >= 0
-    values = torch.where(live, logits.float(), 0.0)
-    p, lse = torch.softmax(values, dim=1), torch.logsumexp(values, dim=1, keepdim=True)
-    grad = torch.zeros_like(p)
-    if dweights is not None:
-        chosen = indices >= 0
-        g = torch.where(chosen, dweights, 0.0)
-        dot = torch.where(chosen, weights * g, 0.0).sum(1, keepdim=True)
-        own = torch.where(chosen, weights * (g - dot if normalize else g), 0.0)
-        grad.scatter_add_(1, indices.clamp_min(0).long(), own)
-        if not normalize:
-            grad -= p * dot
-    if dbalance is not None:
-        share = counts * inverse[1]
-        grad += dbalance * experts * inverse[0] * p * (share - (p * share).sum(1, keepdim=True))
-    if dz is not None:
-        grad += dz * 2.0 * inverse[0] * lse * p
-    return torch.where(live, grad, 0.0).to(logits.dtype)
+    tokens, choices = live.sum().clamp_min(1), counts.sum().clamp_min(1)
+    balance = experts * (counts * torch.where(live[:, None], p, 0.0).sum(0)).sum() / tokens / choices
+    z = torch.where(live, lse * lse, 0.0).sum() / tokens
+    return weights.view(*lead, top_k), indices.to(torch.int32).view(*lead, top_k), counts, balance, z
 
 
 def expert_plan(indices, experts):
-    """Stable counting sort of [tokens, top_k] choices: (offsets int32 [experts + 1], positions int32 [tokens, top_k])."""
     flat = indices.reshape(-1).long()
     bins = torch.where((flat >= 0) & (flat < experts), flat, experts)
     offsets = torch.zeros(experts + 1, dtype=torch.int32)
     offsets[1:] = torch.bincount(bins, minlength=experts + 1)[:experts].cumsum(0)
     positions = torch.empty_like(flat)
     positions[bins.argsort(stable=True)] = torch.arange(flat.numel())
-    return offsets, torch.where(bins < experts, positions, -1).to(torch.int32).view(indices.shape)
+    return offsets, torch.where(bins < experts, positions, -1).to(torch.int32).view(-1, indices.shape[-1])
 
 
-def _placed(positions, capacity):
+def _placed(positions):
+    capacity = positions.numel()
     return (positions >= 0) & (positions < capacity), positions.clamp(0, max(0, capacity - 1)).long()
 
 
 def expert_dispatch(x, positions, offsets):
-    capacity = positions.numel()
-    rows = x.new_zeros((capacity, x.shape[1]))
-    placed, _ = _placed(positions, capacity)
-    token, choice = placed.nonzero(as_tuple=True)
-    rows[positions[token, choice].long()] = x[token]
-    return rows
+    flat = x.reshape(-1, x.shape[-1]).float()
+    placed, at = _placed(positions)
+    token = placed.nonzero(as_tuple=True)[0]
+    rows = flat.new_zeros((positions.numel(), flat.shape[1]))
+    return rows.index_put((at[placed],), flat[token]).to(x.dtype)
 
 
-def expert_combine(rows, positions, weights=None):
-    if not positions.numel():
-        return rows.new_zeros((positions.shape[0], rows.shape[1]))
-    placed, at = _placed(positions, rows.shape[0])
-    factor = placed.float() if weights is None else torch.where(placed, weights.float().view(positions.shape), 0.0)
+def expert_combine(rows, weights, positions, offsets):
+    placed, at = _placed(positions)
+    factor = torch.where(placed, weights.float().reshape(positions.shape), 0.0)
     values = torch.where(placed[..., None], rows.float()[at], 0.0)
-    return (values * factor[..., None]).sum(1).to(rows.dtype)
-
-
-def expert_combine_backward(dout, rows, positions, offsets, weights):
-    placed, at = _placed(positions, rows.shape[0])
-    drows = torch.zeros_like(rows)
-    dweights = torch.zeros_like(weights)
-    if positions.numel():
-        grad = dout.float()[:, None] * weights.float().view(positions.shape)[..., None]
-        drows[at[placed]] = grad[placed].to(rows.dtype)
-        dot = torch.where(placed, (rows.float()[at] * dout.float()[:, None]).sum(2), 0.0)
-        dweights = dot.to(weights.dtype).view(weights.shape)
-    return drows, dweights
+    return (values * factor[..., None]).sum(1).to(rows.dtype).view(*weights.shape[:-1], rows.shape[1])
 
 
 # --------------------------------------------------------------------------- RMS norms around a block
-def _per_row(vector, rows, tokens, shift=0.0):
-    """fp32 [rows, cols] (or [1, cols]) factors of an optional shared / per-sample vector."""
-    if vector is None:
-        return 1.0
-    value = vector.float() + shift
-    return value if vector.dim() == 1 else value.repeat_interleave(tokens, dim=0)
+def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
+    width = x.shape[-1]
 
-
-def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, *, residual_scale=1.0, eps=1e-6, h_dtype=None):
-    """Forward of :func:`viola_b200.ops.block_norm`: (out, h, ry, ru), None for what was not asked for."""
-    rows = x.shape[0]
-    u, out, h, ry, ru = x.float(), None, None, None, None
-    if y is not None:
-        value = y.float()
-        ry = torch.rsqrt((value * value).mean(1) + eps)
-        u = residual_scale * u + value * ry[:, None] * _per_row(weight, rows, tokens) * _per_row(gate, rows, tokens)
-        out = u.to(x.dtype)
-    if h_dtype is not None:
-        ru = torch.rsqrt((u * u).mean(1) + eps)
-        h = (u * ru[:, None] * _per_row(next_weight, rows, tokens) * _per_row(next_scale, rows, tokens, 1.0)).to(h_dtype)
-    return out, h, ry, ru
-
-
-def block_norm_backward(x, y, weight, gate, next_weight, next_scale, tokens, ry, ru, dout, dh, *, residual_scale=1.0):
-    """(dx, dy, dweight, dgate, dnext_weight, dnext_scale); None where there is nothing to differentiate."""
-    rows, cols = x.shape
-    samples = rows // tokens
-
-    def sums(value, vector, other):
+    def factor(vector, shift=0.0):
         if vector is None:
-            return None
-        value = value * other
-        value = value.sum(0) if vector.dim() == 1 else value.view(samples, tokens, cols).sum(1)
-        return value.to(vector.dtype)
+            return 1.0
+        value = vector.contiguous().float() + shift
+        return value if vector.dim() == 1 else value[:, None]
 
-    d = dout.float() if dout is not None else torch.zeros((rows, cols))
-    u, dy, dweight, dgate, dnext_weight, dnext_scale = x.float(), None, None, None, None, None
+    def unit(v):
+        return v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps)
+
+    u, results = x.contiguous().view(-1, tokens, width).float(), []
     if y is not None:
-        w, g = _per_row(weight, rows, tokens), _per_row(gate, rows, tokens)
-        yh = y.float() * ry[:, None]
-        u = residual_scale * u + yh * w * g
-    if dh is not None:
-        w2, s2 = _per_row(next_weight, rows, tokens), _per_row(next_scale, rows, tokens, 1.0)
-        uh, grad = u * ru[:, None], dh.float()
-        dnext_weight, dnext_scale = sums(grad * uh, next_weight, s2), sums(grad * uh, next_scale, w2)
-        t = grad * w2 * s2
-        d = d + ru[:, None] * (t - uh * (t * uh).mean(1, keepdim=True))
-    if y is not None:
-        dweight, dgate = sums(d * yh, weight, g), sums(d * yh, gate, w)
-        t = d * w * g
-        dy = (ry[:, None] * (t - yh * (t * yh).mean(1, keepdim=True))).to(y.dtype)
-        d = residual_scale * d
-    return d.to(x.dtype), dy, dweight, dgate, dnext_weight, dnext_scale
+        u = residual_scale * u + unit(y.contiguous().view(-1, tokens, width).float()) * factor(weight) * factor(gate)
+        results.append(u.to(x.dtype).view(x.shape))
+    if h_dtype is not None:
+        results.append((unit(u) * factor(next_weight) * factor(next_scale, 1.0)).to(h_dtype).view(x.shape))
+    return results
