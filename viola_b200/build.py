@@ -26,7 +26,7 @@ CPP_SOURCES = ["bindings.cpp", "functions.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default",
+    "--expt-relaxed-constexpr", "--split-compile=0", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default",
 ]
 
 
