@@ -152,6 +152,15 @@ def test_route_passes_nan_on_with_indices_in_range(device):
     assert out.balance_loss.isnan() and out.z_loss.isnan() | out.z_loss.isinf()
 
 
+def test_route_with_an_infinite_bias(device):
+    """+inf puts an expert first and -inf last, but neither opens a closed expert or a masked token."""
+    logits = torch.tensor([[0.0, 1.0, 2.0, -math.inf], [5.0, 4.0, 3.0, 2.0], [0.0, 0.0, 0.0, 0.0]], device=device)
+    bias = torch.tensor([math.inf, 0.0, -math.inf, math.inf], device=device)
+    out = nn.route_tokens(logits, 3, bias=bias, mask=torch.tensor([True, True, False], device=device))
+    assert out.indices.tolist() == [[0, 1, -1], [0, 3, 1], [-1, -1, -1]] and out.counts.tolist() == [2, 2, 0, 1]
+    torch.testing.assert_close(out.weights[1].cpu(), torch.softmax(torch.tensor([5.0, 2.0, 4.0]), 0), rtol=1e-6, atol=0)
+
+
 def test_route_shapes_strides_and_no_tokens(device):
     base = randn(3, 2, 7, 24, dtype=BF16).to(device)
     logits = base[..., ::2]                                    # strided columns

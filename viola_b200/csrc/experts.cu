@@ -73,28 +73,44 @@ __device__ __forceinline__ void store_values(T* row, int sub, int experts, bool 
   }
 }
 
+// shared memory words of a warp's lists in the forward pass, V keys a lane
+__host__ __device__ constexpr int route_list_words(int v) { return ((v + 4) / 4 * 4 + (v + 3) / 4 * 4) * 32 + 64; }
+
 template <int G> __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   return v;
 }
 template <int G> __device__ __forceinline__ float group_max(float v) {
+  if constexpr (G == 32) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+  }
 #pragma unroll
   for (int o = G / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
 
-// Unsigned integers in the order of the keys: -inf is 0 (never chosen), NaN the largest (as a descending sort has it).
+// Unsigned integers in the order of the keys.  A key comes out of an addition, which leaves neither -0 (the bias is never
+// -0) nor a NaN with the sign set: NaN is the largest, as a descending sort has it, and nothing is below -inf.  Keys of
+// -inf are never chosen, and kTaken marks those that have been.
+constexpr unsigned kTaken = 0u, kClosed = 0x007fffffu;       // kClosed: ordered(-inf)
 __device__ __forceinline__ unsigned ordered(float key) {
-  if (key != key) return 0xffffffffu;
-  if (key == -INFINITY) return 0u;
-  const unsigned bits = __float_as_uint(key + 0.0f);       // -0 + 0 = +0: the two zeros tie
-  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+  const unsigned bits = __float_as_uint(key);
+  return bits ^ ((unsigned)((int)bits >> 31) | 0x80000000u);
 }
 
-// softmax of a row: p[i], and its log-sum-exp
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// e[i] = exp(l[i] - top) with top the row's maximum; returns their sum.  The hardware's base-2 exponential is off by about
+// 2^-22 of its value and its argument by 2^-24 |l - top|, a few steps of fp32 where p is not negligible.
 template <int G, int V>
-__device__ __forceinline__ float group_softmax(const float (&l)[V], float (&p)[V], float& top, float& total) {
+__device__ __forceinline__ float group_exp(const float (&l)[V], float (&e)[V], float& top) {
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < V; ++i) m = fmaxf(m, l[i]);
@@ -102,14 +118,10 @@ __device__ __forceinline__ float group_softmax(const float (&l)[V], float (&p)[V
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    p[i] = expf(l[i] - top);
-    s += p[i];
+    e[i] = exp2_fast((l[i] - top) * 1.4426950408889634f);
+    s += e[i];
   }
-  total = group_sum<G>(s);
-  const float inverse = 1.f / total;
-#pragma unroll
-  for (int i = 0; i < V; ++i) p[i] *= inverse;
-  return top + logf(total);
+  return group_sum<G>(s);
 }
 
 struct RouteArgs {
@@ -127,64 +139,73 @@ struct RouteArgs {
   float* partial;              // [blocks][2 * experts + 2]: sums of p, counts, sum of lse^2, tokens
 };
 
-// balance = E * sum_e (counts_e / choices) * (sum_t p_te / tokens) from per-expert totals in shared memory
-__device__ __forceinline__ void route_finish(const RouteArgs& a, const float* p_sum, const int* count, float z, int tokens) {
-  __shared__ float dot_part[32];
-  __shared__ int sum_part[32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  float dot = 0.f;
-  int sum = 0;
-  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
-    dot = fmaf((float)count[e], p_sum[e], dot);
-    sum += count[e];
-    a.counts[e] = count[e];
-  }
-  dot = group_sum<32>(dot);
-  sum = __reduce_add_sync(kFull, sum);
-  if (lane == 0) {
-    dot_part[warp] = dot;
-    sum_part[warp] = sum;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    dot = 0.f;
-    sum = 0;
-    for (int w = 0; w < warps; ++w) {
-      dot += dot_part[w];
-      sum += sum_part[w];
-    }
-    const float per_token = 1.f / (float)max(tokens, 1), per_choice = 1.f / (float)max(sum, 1);
-    *a.balance = (float)a.experts * dot * per_token * per_choice;
-    *a.z = z * per_token;
-    a.inverse[0] = per_token;
-    a.inverse[1] = per_choice;
-  }
+// The losses of a batch from dot = sum_e counts_e sum_t p_te, choices = sum_e counts_e, z = sum of lse^2 and the tokens.
+__device__ __forceinline__ void route_losses(const RouteArgs& a, float dot, int choices, float z, int tokens) {
+  const float per_token = 1.f / (float)max(tokens, 1), per_choice = 1.f / (float)max(choices, 1);
+  *a.balance = (float)a.experts * dot * per_token * per_choice;
+  *a.z = z * per_token;
+  a.inverse[0] = per_token;
+  a.inverse[1] = per_choice;
 }
 
+// Sorts a lane's keys, largest first: Batcher's odd-even merge sort, 19 exchanges for 8 keys, 63 for 16.
+template <int V> __device__ __forceinline__ void sort_keys(unsigned (&key)[V]) {
+#pragma unroll
+  for (int p = 1; p < V; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < V; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < V && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const unsigned high = max(key[i + j], key[i + j + k]);
+            key[i + j + k] = min(key[i + j], key[i + j + k]);
+            key[i + j] = high;
+          }
+}
+
+// A lane sorts its (up to 16) keys; each choice then costs one maximum over the token's lanes and one step down the winner's
+// list in shared memory, and which expert a winning key belongs to is looked up for all choices at once.  More keys than
+// that are searched again for every choice.
+// Bound by the instructions it issues, most of them the same for a token whatever its experts: 16 lanes to a token put two
+// tokens into each.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256)
 route_forward_kernel(const RouteArgs a) {
-  extern __shared__ float shared[];             // [8][experts] sums of p, [experts] counts
-  __shared__ float z_part[8];
-  __shared__ int n_part[8];
+  constexpr int kWarps = 8, kThreads = kWarps * 32;
   constexpr int kTokens = 32 / G;               // tokens a warp serves at a time
+  constexpr bool kSorted = V > 1 && V <= 16;
+  // [experts] counts, [G * V] bias; then per warp, by lane, [V + 1][32] keys in descending order, [32][V] keys as they come,
+  // [32] winning keys and [32] their lanes; in the end in their place [warps][experts] sums of p
+  extern __shared__ __align__(16) unsigned char route_shared[];
+  int* count = reinterpret_cast<int*>(route_shared);
+  float* bias = reinterpret_cast<float*>(route_shared + (a.experts + 3) / 4 * 16);
+  float* shared = bias + G * V;
+  __shared__ float z_part[kWarps], dot_part[kWarps];
+  __shared__ int n_part[kWarps], sum_part[kWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (G - 1), base = lane - sub;
-  int* count = reinterpret_cast<int*>(shared + 8 * a.experts);
-  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) count[e] = 0;
+  unsigned* lists = reinterpret_cast<unsigned*>(shared) + warp * route_list_words(V) + lane;      // [place * 32]
+  uint4* keys = reinterpret_cast<uint4*>(lists - lane + (V + 4) / 4 * 4 * 32);                    // [word * 32 + lane]
+  unsigned* winners = lists - lane + route_list_words(V) - 64;                                   // [32] keys, [32] lanes
+  for (int e = threadIdx.x; e < G * V; e += kThreads) {
+    if (e < a.experts) count[e] = 0;
+    // +inf (and NaN) as the largest number, so that a logit of -inf stays closed; -0 as 0
+    const float b = a.bias != nullptr && e < a.experts ? a.bias[e] : 0.f;
+    bias[e] = b < INFINITY ? b + 0.f : 3.402823466e+38f;
+  }
   __syncthreads();
 
-  float bias[V], p_sum[V], z_sum = 0.f;
+  float p_sum[V], z_sum = 0.f;
   int live_tokens = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    bias[i] = a.bias != nullptr && sub * V + i < a.experts ? a.bias[sub * V + i] : 0.f;
-    p_sum[i] = 0.f;
-  }
-  for (long long first = (long long)(blockIdx.x * 8 + warp) * kTokens; first < a.tokens;
-       first += (long long)gridDim.x * 8 * kTokens) {
+  for (int i = 0; i < V; ++i) p_sum[i] = 0.f;
+  if constexpr (kSorted) lists[V * 32] = kTaken;                                // the end of every list
+  for (long long first = (long long)(blockIdx.x * kWarps + warp) * kTokens; first < a.tokens;
+       first += (long long)gridDim.x * kThreads / G) {
     const long long token = first + lane / G;
     const bool inside = token < a.tokens, live = inside && (a.mask == nullptr || a.mask[token] != 0);
-    float l[V], p[V], top, total;
+    float l[V], e[V], top;
     unsigned key[V];
     if (live) {
       load_values<T, G, V>(reinterpret_cast<const T*>(a.logits) + token * a.stride, sub, a.experts, a.wide, l);
@@ -193,59 +214,99 @@ route_forward_kernel(const RouteArgs a) {
       for (int i = 0; i < V; ++i) l[i] = -INFINITY;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) key[i] = sub * V + i < a.experts ? ordered(l[i] + bias[i]) : 0u;
-    const float lse = group_softmax<G, V>(l, p, top, total);
+    for (int i = 0; i < V; ++i) key[i] = ordered(l[i] + bias[sub * V + i]);
+    const float total = group_exp<G, V>(l, e, top);
 
     int my_index = -1;
-    float my_logit = -INFINITY;
-    for (int j = 0; j < a.top_k; ++j) {
-      unsigned best = 0u;
-      int at = INT_MAX;
-      float logit = 0.f;
+    if constexpr (kSorted) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (key[i] > best) {                    // strictly: the lowest index of equal keys stays
-          best = key[i];
-          at = sub * V + i;
-          logit = l[i];
-        }
-      }
-      int index;
-      if constexpr (G == 32) {
-        const unsigned most = __reduce_max_sync(kFull, best);
-        index = most == 0u ? -1 : (int)__reduce_min_sync(kFull, best == most ? (unsigned)at : (unsigned)INT_MAX);
-      } else {
+      for (int w = 0; w < (V + 3) / 4; ++w)
+        keys[w * 32 + lane] = make_uint4(key[4 * w], 4 * w + 1 < V ? key[4 * w + 1 < V ? 4 * w + 1 : 0] : kTaken,
+                                         4 * w + 2 < V ? key[4 * w + 2 < V ? 4 * w + 2 : 0] : kTaken,
+                                         4 * w + 3 < V ? key[4 * w + 3 < V ? 4 * w + 3 : 0] : kTaken);
+      sort_keys<V>(key);
+#pragma unroll
+      for (int i = 0; i < V; ++i) lists[i * 32] = key[i];
+      unsigned best = key[0];
+      int place = 0, found = 0;
+      for (int j = 0; j < a.top_k; ++j) {
         unsigned most = best;
-        index = at;
+        if constexpr (G == 32) {
+          most = __reduce_max_sync(kFull, best);
+        } else {
 #pragma unroll
-        for (int o = G / 2; o > 0; o >>= 1) {
-          const unsigned other = __shfl_xor_sync(kFull, most, o);
-          const int other_at = __shfl_xor_sync(kFull, index, o);
-          if (other > most || (other == most && other_at < index)) {
-            most = other;
-            index = other_at;
-          }
+          for (int o = G / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kFull, most, o));
         }
-        if (most == 0u) index = -1;
+        // lanes own ascending experts, so the lowest lane with the largest key has the lowest index among equals
+        const unsigned holders = __ballot_sync(kFull, best == most) >> base & (G == 32 ? kFull : (1u << G) - 1u);
+        const int owner = __ffs(holders) - 1;
+        const bool open = most > kClosed;        // no list is at its end before a key of -inf wins
+        if (sub == j) {
+          winners[lane] = most;
+          winners[32 + lane] = base + owner;
+        }
+        found += open ? 1 : 0;
+        place += open && sub == owner ? 32 : 0;
+        best = lists[place];
       }
-      const float chosen = __shfl_sync(kFull, logit, base + max(index, 0) / V);
-      if (index >= 0 && sub == j) {
-        my_index = index;
-        my_logit = chosen;
-      }
+      // which of its lane's keys the winner is: the first that equals it, or the next ones where the lane won with equal
+      // keys.  A lane without a choice asks for a key that nothing equals, each its own.
+      __syncwarp();
+      const bool asks = sub < found;
+      const unsigned winner = asks ? winners[lane] : kTaken;
+      const int from = asks ? (int)winners[32 + lane] : lane;
+      const unsigned equals = __match_any_sync(kFull, (unsigned long long)winner << 32 | (asks ? from : 32 + lane));
+      int skip = __popc(equals & ((1u << lane) - 1u)), at = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (sub * V + i == index) key[i] = 0u;
+      for (int w = 0; w < (V + 3) / 4; ++w) {
+        const uint4 word = keys[w * 32 + from];
+        const unsigned v[4] = {word.x, word.y, word.z, word.w};
+#pragma unroll
+        for (int i = 0; i < 4 && w * 4 + i < V; ++i) {
+          const bool equal = v[i] == winner;
+          at = equal && skip == 0 ? w * 4 + i : at;
+          skip -= equal ? 1 : 0;
+        }
+      }
+      if (asks) my_index = (from - base) * V + at;
+      __syncwarp();                              // the places are written again for the next token
+    } else {
+      for (int j = 0; j < a.top_k; ++j) {
+        unsigned best = key[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = max(best, key[i]);
+        unsigned most;
+        if constexpr (G == 32) {
+          most = __reduce_max_sync(kFull, best);
+        } else {
+          most = best;
+#pragma unroll
+          for (int o = G / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(kFull, most, o));
+        }
+        const unsigned holders = __ballot_sync(kFull, best == most) >> base & (G == 32 ? kFull : (1u << G) - 1u);
+        const int owner = __ffs(holders) - 1;    // as above
+        int at = 0;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i)
+          if (key[i] == most) at = i;
+        const int chosen = owner * V + __shfl_sync(kFull, at, base + owner);
+        if (sub == j && most > kClosed) my_index = chosen;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (sub * V + i == chosen) key[i] = kTaken;
+      }
     }
 
     const bool counted = __shfl_sync(kFull, my_index, base) >= 0;
+    // the row has just been read: the chosen logits come from the cache
+    const float logit = my_index >= 0 ? to_float(reinterpret_cast<const T*>(a.logits)[token * a.stride + my_index]) : -INFINITY;
     float weight;
     if (a.normalize) {                          // softmax over the chosen logits = p / (sum of the chosen p)
-      const float most = group_max<G>(my_logit);
-      const float e = my_index >= 0 ? expf(my_logit - most) : 0.f;
-      weight = e / group_sum<G>(e);
+      const float most = group_max<G>(logit);
+      const float part = my_index >= 0 ? expf(logit - most) : 0.f;
+      weight = part / group_sum<G>(part);
     } else {
-      weight = expf(my_logit - top) / total;
+      weight = expf(logit - top) / total;
     }
     if (inside && sub < a.top_k) {
       a.indices[token * a.top_k + sub] = my_index;
@@ -253,8 +314,9 @@ route_forward_kernel(const RouteArgs a) {
       if (my_index >= 0) atomicAdd(&count[my_index], 1);
     }
     if (counted) {
+      const float inverse = 1.f / total, lse = top + logf(total);
 #pragma unroll
-      for (int i = 0; i < V; ++i) p_sum[i] += p[i];
+      for (int i = 0; i < V; ++i) p_sum[i] = fmaf(e[i], inverse, p_sum[i]);
       if (sub == 0) {
         z_sum = fmaf(lse, lse, z_sum);
         ++live_tokens;
@@ -262,6 +324,7 @@ route_forward_kernel(const RouteArgs a) {
     }
   }
 
+  __syncthreads();                              // the lists are done with
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
@@ -275,73 +338,125 @@ route_forward_kernel(const RouteArgs a) {
     n_part[warp] = live_tokens;
   }
   __syncthreads();
-  float z = 0.f;
-  int n = 0;
-  for (int w = 0; w < 8; ++w) {
-    z += z_part[w];
-    n += n_part[w];
-  }
   float* mine = a.partial + (long long)blockIdx.x * (2 * a.experts + 2);
-  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+  float dot = 0.f;
+  int choices = 0;
+  for (int e = threadIdx.x; e < a.experts; e += kThreads) {
     float total = 0.f;
-    for (int w = 0; w < 8; ++w) total += shared[w * a.experts + e];
+    for (int w = 0; w < kWarps; ++w) total += shared[w * a.experts + e];
     if (gridDim.x > 1) {
       mine[e] = total;
       mine[a.experts + e] = __int_as_float(count[e]);
     } else {
-      shared[e] = total;                        // column e is read and written by this thread alone
+      a.counts[e] = count[e];
+      dot = fmaf((float)count[e], total, dot);
+      choices += count[e];
     }
   }
-  if (gridDim.x > 1) {
-    if (threadIdx.x == 0) {
+  if (gridDim.x == 1) {
+    dot = group_sum<32>(dot);
+    choices = __reduce_add_sync(kFull, choices);
+    if (lane == 0) {
+      dot_part[warp] = dot;
+      sum_part[warp] = choices;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    float z = 0.f;
+    int n = 0;
+    dot = 0.f;
+    choices = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      z += z_part[w];
+      n += n_part[w];
+      if (gridDim.x == 1) {
+        dot += dot_part[w];
+        choices += sum_part[w];
+      }
+    }
+    if (gridDim.x == 1) {
+      route_losses(a, dot, choices, z, n);
+    } else {
       mine[2 * a.experts] = z;
       mine[2 * a.experts + 1] = __int_as_float(n);
     }
-    return;
   }
-  __syncthreads();
-  route_finish(a, shared, count, z, n);
 }
 
-// Adds the blocks' sums in block order and derives the losses: 1024 threads, `experts` rounded up to a power of two
-// columns x as many interleaved row groups as fit.
-__global__ void __launch_bounds__(1024)
-route_finish_kernel(const RouteArgs a, int blocks, int columns) {
-  extern __shared__ float shared[];             // [groups][columns] sums, [groups][columns] counts
-  const int groups = 1024 / columns, column = threadIdx.x % columns, group = threadIdx.x / columns;
-  int* counts = reinterpret_cast<int*>(shared + 1024);
-  const int pitch = 2 * a.experts + 2;
-  float p = 0.f;
-  int c = 0;
-  if (column < a.experts) {
-    for (int b = group; b < blocks; b += groups) {
-      p += a.partial[(long long)b * pitch + column];
-      c += __float_as_int(a.partial[(long long)b * pitch + a.experts + column]);
+// Adds the blocks' sums in block order and derives the losses: one cluster, each block of which takes every eighth set of
+// 32 experts with 32 threads per expert; the first block adds the clusters' shares of the balance in order.
+constexpr int kFinishBlocks = 8;
+__global__ void __cluster_dims__(kFinishBlocks, 1, 1) __launch_bounds__(1024)
+route_finish_kernel(const RouteArgs a, int blocks) {
+  __shared__ float p_part[32][33];
+  __shared__ int c_part[32][33];
+  __shared__ float share[2];                    // this block's part of dot, and of choices as bits
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
+  const long long pitch = 2 * a.experts + 2;
+  float dot = 0.f;
+  int choices = 0;
+  for (int first = blockIdx.x * 32; first < a.experts; first += kFinishBlocks * 32) {
+    const int e = first + lane;
+    float p = 0.f;
+    int c = 0;
+    if (e < a.experts) {
+#pragma unroll 4
+      for (int b = row; b < blocks; b += 32) {
+        p += a.partial[b * pitch + e];
+        c += __float_as_int(a.partial[b * pitch + a.experts + e]);
+      }
     }
+    p_part[row][lane] = p;
+    c_part[row][lane] = c;
+    __syncthreads();
+    if (row == 0) {
+      p = 0.f;
+      c = 0;
+#pragma unroll 8
+      for (int r = 0; r < 32; ++r) {
+        p += p_part[r][lane];
+        c += c_part[r][lane];
+      }
+      if (e < a.experts) a.counts[e] = c;
+      dot += group_sum<32>((float)c * p);
+      choices += __reduce_add_sync(kFull, c);
+    }
+    __syncthreads();
   }
-  shared[group * columns + column] = p;
-  counts[group * columns + column] = c;
   float z = 0.f;
   int n = 0;
-  if (threadIdx.x < 32) {
-    for (int b = threadIdx.x; b < blocks; b += 32) {
-      z += a.partial[(long long)b * pitch + 2 * a.experts];
-      n += __float_as_int(a.partial[(long long)b * pitch + 2 * a.experts + 1]);
+  if (blockIdx.x == 0 && row == 0) {
+#pragma unroll 4
+    for (int b = lane; b < blocks; b += 32) {
+      z += a.partial[b * pitch + 2 * a.experts];
+      n += __float_as_int(a.partial[b * pitch + 2 * a.experts + 1]);
     }
     z = group_sum<32>(z);
     n = __reduce_add_sync(kFull, n);
   }
-  __syncthreads();
-  if (group == 0) {
-    for (int g = 1; g < groups; ++g) {
-      p += shared[g * columns + column];
-      c += counts[g * columns + column];
-    }
-    shared[column] = p;
-    counts[column] = c;
+  if (threadIdx.x == 0) {
+    share[0] = dot;
+    share[1] = __int_as_float(choices);
   }
-  __syncthreads();
-  route_finish(a, shared, counts, z, n);
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    dot = 0.f;
+    choices = 0;
+    for (int b = 0; b < kFinishBlocks; ++b) {
+      const uint32_t here = (uint32_t)__cvta_generic_to_shared(share);
+      uint32_t there;
+      float part, sum;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(b));
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part) : "r"(there) : "memory");
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(sum) : "r"(there + 4) : "memory");
+      dot += part;
+      choices += __float_as_int(sum);
+    }
+    route_losses(a, dot, choices, z, n);
+  }
+  // the others' shared memory stays until it has been read
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 struct RouteBackwardArgs {
@@ -367,7 +482,11 @@ template <typename T, int G, int V>
 __global__ void __launch_bounds__(256)
 route_backward_kernel(const RouteBackwardArgs a) {
   constexpr int kTokens = 32 / G;
+  __shared__ float chosen_grad[8][32 * V];      // of the tokens that a warp works on, zero where not chosen
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (G - 1), base = lane - sub;
+  float* mine = chosen_grad[warp] + base * V;
+  for (int i = lane; i < 32 * V; i += 32) chosen_grad[warp][i] = 0.f;
+  __syncwarp();
   const float per_token = a.inverse[0], per_choice = a.inverse[1];
   const float cb = a.dbalance != nullptr ? *a.dbalance * (float)a.experts * per_token : 0.f;
   const float cz = a.dz != nullptr ? *a.dz * 2.f * per_token : 0.f;
@@ -387,17 +506,20 @@ route_backward_kernel(const RouteBackwardArgs a) {
       if (index < 0) w = g = 0.f;
     }
     const bool counted = __shfl_sync(kFull, index, base) >= 0;
-    float l[V], p[V], top, total;
+    float l[V], p[V], top;
     if (counted) {
       load_values<T, G, V>(reinterpret_cast<const T*>(a.logits) + token * a.stride, sub, a.experts, a.wide, l);
     } else {
 #pragma unroll
       for (int i = 0; i < V; ++i) l[i] = -INFINITY;
     }
-    const float lse = group_softmax<G, V>(l, p, top, total);
+    const float total = group_exp<G, V>(l, p, top), lse = top + logf(total), inverse = 1.f / total;
     float pf = 0.f;
 #pragma unroll
-    for (int i = 0; i < V; ++i) pf = fmaf(p[i], f[i], pf);
+    for (int i = 0; i < V; ++i) {
+      p[i] *= inverse;
+      pf = fmaf(p[i], f[i], pf);
+    }
     pf = group_sum<G>(pf);
     const float dot = group_sum<G>(w * g);
     const float common = cz * lse - (a.normalize ? 0.f : dot);
@@ -405,13 +527,13 @@ route_backward_kernel(const RouteBackwardArgs a) {
     float grad[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) grad[i] = p[i] * fmaf(cb, f[i] - pf, common);
-    for (int j = 0; j < a.top_k; ++j) {
-      const int at = __shfl_sync(kFull, index, base + j);
-      const float add = __shfl_sync(kFull, own, base + j);
+    if (index >= 0) mine[index] = own;
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (sub * V + i == at) grad[i] += add;
-    }
+    for (int i = 0; i < V; ++i) grad[i] += mine[sub * V + i];
+    __syncwarp();
+    if (index >= 0) mine[index] = 0.f;
+    __syncwarp();
     if (inside) {
       if (!counted) {
 #pragma unroll
@@ -691,43 +813,52 @@ using namespace vb;
 
 static bool aligned_to(const void* p, long long bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
-// lanes per token and experts per lane
-#define VB_ROUTE_SWITCH(experts, ...)                                            \
-  if ((experts) <= 4) { constexpr int G = 4, V = 1; __VA_ARGS__; }               \
-  else if ((experts) <= 8) { constexpr int G = 8, V = 1; __VA_ARGS__; }          \
-  else if ((experts) <= 16) { constexpr int G = 16, V = 1; __VA_ARGS__; }        \
-  else if ((experts) <= 32) { constexpr int G = 32, V = 1; __VA_ARGS__; }        \
-  else if ((experts) <= 64) { constexpr int G = 32, V = 2; __VA_ARGS__; }        \
-  else if ((experts) <= 128) { constexpr int G = 32, V = 4; __VA_ARGS__; }       \
-  else if ((experts) <= 256) { constexpr int G = 32, V = 8; __VA_ARGS__; }       \
-  else if ((experts) <= 512) { constexpr int G = 32, V = 16; __VA_ARGS__; }      \
-  else { constexpr int G = 32, V = 32; __VA_ARGS__; }
+// lanes per token (G) and experts per lane (V)
+#define VB_ROUTE_CASE(g, v, ...) if (lanes == g && per_lane == v) { constexpr int G = g, V = v; __VA_ARGS__; }
+#define VB_ROUTE_SWITCH(...)                                                                     \
+  VB_ROUTE_CASE(4, 1, __VA_ARGS__) else VB_ROUTE_CASE(8, 1, __VA_ARGS__)                         \
+  else VB_ROUTE_CASE(16, 1, __VA_ARGS__) else VB_ROUTE_CASE(16, 2, __VA_ARGS__)                  \
+  else VB_ROUTE_CASE(16, 4, __VA_ARGS__) else VB_ROUTE_CASE(16, 8, __VA_ARGS__)                  \
+  else VB_ROUTE_CASE(16, 16, __VA_ARGS__) else VB_ROUTE_CASE(32, 1, __VA_ARGS__)                 \
+  else VB_ROUTE_CASE(32, 2, __VA_ARGS__) else VB_ROUTE_CASE(32, 4, __VA_ARGS__)                  \
+  else VB_ROUTE_CASE(32, 8, __VA_ARGS__) else VB_ROUTE_CASE(32, 16, __VA_ARGS__)                 \
+  else VB_ROUTE_CASE(32, 32, __VA_ARGS__)
 
 #define VB_FLOAT_SWITCH(dtype, ...)                                              \
   if ((dtype) == kF32) { using T = float; __VA_ARGS__; }                         \
   else if ((dtype) == kBF16) { using T = __nv_bfloat16; __VA_ARGS__; }           \
   else { using T = __half; __VA_ARGS__; }
 
-static int route_lanes(int experts) { return experts <= 4 ? 4 : experts <= 8 ? 8 : experts <= 16 ? 16 : 32; }
-// blocks of 8 warps
-static int route_blocks(int tokens, int experts) {
-  const long long per_pass = 8LL * (32 / route_lanes(experts));
-  if (tokens <= 4 * per_pass) return 1;
-  return (int)std::min<long long>((tokens + per_pass - 1) / per_pass, 148LL * 2);
+// A token's lanes hold one choice each at the end, so there are at least top_k of them.
+static int route_lanes(int experts, int top_k) {
+  if (experts <= 16) return experts <= 4 ? 4 : experts <= 8 ? 8 : 16;
+  return top_k <= 16 && experts <= 256 ? 16 : 32;
 }
-static bool route_wide(const void* p, long long stride, int experts, int size) {
-  const int lanes = route_lanes(experts), per_lane = experts / lanes;
-  if (experts % lanes || (per_lane & (per_lane - 1))) return false;
+static int route_per_lane(int experts, int lanes) {
+  int v = 1;
+  while (v * lanes < experts) v *= 2;
+  return v;
+}
+// Blocks (of 8 warps) of the forward pass: one where it makes no more than four passes, else at most four per SM
+static int route_blocks(int tokens, int lanes) {
+  const long long per_pass = 8LL * (32 / lanes);
+  if (tokens <= 4 * per_pass) return 1;
+  return (int)std::min<long long>((tokens + per_pass - 1) / per_pass, 148LL * 4);
+}
+static bool route_wide(const void* p, long long stride, int experts, int lanes, int per_lane, int size) {
   const int bytes = std::min(16, per_lane * size);
-  return aligned_to(p, bytes) && stride * size % bytes == 0;
+  return experts == lanes * per_lane && aligned_to(p, bytes) && stride * size % bytes == 0;
 }
 static bool route_shape_ok(int tokens, int experts, int top_k, int dtype) {
   return tokens >= 0 && experts >= 1 && experts <= kMaxExperts && top_k >= 1 && top_k <= std::min(experts, kMaxTopK) &&
          dtype >= kF32 && dtype <= kF16;
 }
 
+// (for any top_k: 16 lanes make the fewest tokens per pass for short batches, 32 the most blocks)
 extern "C" long long vb_route_workspace(int tokens, int experts) {
-  return tokens < 0 || experts < 1 ? 0 : (long long)route_blocks(tokens, experts) * (2 * experts + 2);
+  if (tokens < 0 || experts < 1) return 0;
+  return (long long)std::max(route_blocks(tokens, route_lanes(experts, 1)), route_blocks(tokens, route_lanes(experts, kMaxTopK))) *
+         (2 * experts + 2);
 }
 
 extern "C" int vb_route_forward(const void* logits, int dtype, int tokens, int experts, long long stride, const float* bias,
@@ -737,17 +868,15 @@ extern "C" int vb_route_forward(const void* logits, int dtype, int tokens, int e
   if (!route_shape_ok(tokens, experts, top_k, dtype) || workspace == nullptr ||
       workspace_floats < vb_route_workspace(tokens, experts))
     return (int)cudaErrorInvalidValue;
+  const int lanes = route_lanes(experts, top_k), per_lane = route_per_lane(experts, lanes), blocks = route_blocks(tokens, lanes);
   RouteArgs a{logits, stride, tokens, experts, top_k, normalize, 0, bias, mask, weights, indices, counts, balance, z, inverse,
               workspace};
-  a.wide = route_wide(logits, stride, experts, dtype == kF32 ? 4 : 2);
-  const int blocks = route_blocks(tokens, experts);
-  const size_t smem = (size_t)9 * experts * sizeof(float);
-  VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH(experts, (route_forward_kernel<T, G, V><<<blocks, 256, smem, stream>>>(a))));
-  if (blocks > 1) {
-    int columns = 32;
-    while (columns < experts) columns *= 2;
-    route_finish_kernel<<<1, 1024, 2048 * sizeof(float), stream>>>(a, blocks, columns);
-  }
+  a.wide = route_wide(logits, stride, experts, lanes, per_lane, dtype == kF32 ? 4 : 2);
+  const size_t lists = per_lane > 1 && per_lane <= 16 ? 8 * route_list_words(per_lane) * sizeof(int) : 0;
+  // at most 40 KB
+  const size_t smem = ((size_t)(experts + 3) / 4 * 4 + lanes * per_lane) * 4 + std::max(lists, (size_t)8 * experts * sizeof(float));
+  VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_forward_kernel<T, G, V><<<blocks, 256, smem, stream>>>(a))));
+  if (blocks > 1) route_finish_kernel<<<kFinishBlocks, 1024, 0, stream>>>(a, blocks);
   return (int)cudaGetLastError();
 }
 
@@ -757,13 +886,13 @@ extern "C" int vb_route_backward(const void* logits, int dtype, int tokens, int 
                                  void* dlogits, cudaStream_t stream) {
   if (!route_shape_ok(tokens, experts, top_k, dtype)) return (int)cudaErrorInvalidValue;
   if (tokens == 0) return 0;
+  const int lanes = route_lanes(experts, top_k), per_lane = route_per_lane(experts, lanes), size = dtype == kF32 ? 4 : 2;
   RouteBackwardArgs a{logits, stride, tokens, experts, top_k, normalize, 0, weights, indices, counts, inverse, dweights,
                       dbalance, dz, dlogits};
-  const int size = dtype == kF32 ? 4 : 2;
-  a.wide = route_wide(logits, stride, experts, size) && route_wide(dlogits, experts, experts, size);
-  const long long per_pass = 8LL * (32 / route_lanes(experts));
+  a.wide = route_wide(logits, stride, experts, lanes, per_lane, size) && route_wide(dlogits, experts, experts, lanes, per_lane, size);
+  const long long per_pass = 8LL * (32 / lanes);
   const int blocks = (int)std::min<long long>((tokens + per_pass - 1) / per_pass, 148LL * 8);
-  VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH(experts, (route_backward_kernel<T, G, V><<<blocks, 256, 0, stream>>>(a))));
+  VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_backward_kernel<T, G, V><<<blocks, 256, 0, stream>>>(a))));
   return (int)cudaGetLastError();
 }
 

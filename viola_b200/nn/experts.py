@@ -56,7 +56,7 @@ def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
 
     With p the softmax of a token's logits and S its chosen experts, the weights are ``p_e / sum_S p`` (``normalize``) or
     ``p_e``, in fp32 whatever the logits' dtype.  S holds the largest ``fp32(logit) + bias`` (``bias``: optional fp32
-    [experts], it moves the choice and nothing else), the lowest index among equals; an expert whose logit is -inf is never
+    [experts], it moves the choice and nothing else; +inf counts as the largest number), the lowest index among equals; an expert whose logit is -inf is never
     chosen, and slots left over get index -1 and weight 0.  ``mask`` (bool, the leading shape) is False for padding:
     those tokens, like tokens with no logit above -inf, choose nothing and enter no sum whatever their logits hold.
 

@@ -488,7 +488,10 @@ def route(logits, top_k, *, bias=None, mask=None, normalize=True):
     values = logits.reshape(-1, experts).float()
     if mask is not None:
         values = torch.where(mask.reshape(-1, 1), values, -math.inf)
-    key = values.detach() if bias is None else values.detach() + bias.float()
+    key = values.detach()
+    if bias is not None:
+        # a bias of +inf leaves a logit of -inf closed
+        key = key + torch.where(bias < math.inf, bias.float(), torch.finfo(torch.float32).max)
     ranked, order = key.sort(dim=1, descending=True, stable=True)
     indices = torch.where(ranked[:, :top_k] == -math.inf, -1, order[:, :top_k])
     chosen = indices >= 0
