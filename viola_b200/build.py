@@ -21,12 +21,13 @@ CSRC = ROOT / "csrc"
 OBJ = ROOT / "build"
 TARGET = ROOT / "_C.so"
 
-CUDA_SOURCES = ["quant.cu", "gemm_sm100.cu", "mxfp8_gemm_sm100.cu", "attention_sm100.cu", "optim.cu", "codec.cu", "comm.cu", "fused.cu", "experts.cu", "block_norm.cu", "multi.cu", "noalloc.cu"]
+CUDA_SOURCES = ["quant.cu", "gemm_sm100.cu", "mxfp8_gemm_sm100.cu", "attention_sm100.cu", "optim.cu", "codec.cu", "comm.cu", "fused.cu", "experts.cu", "block_norm.cu", "block_norm_f32.cu", "block_norm_f32_bf16.cu", "block_norm_f32_f16.cu", "block_norm_bf16.cu",
+                "block_norm_f16.cu", "multi.cu", "noalloc.cu"]
 CPP_SOURCES = ["bindings.cpp", "functions.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "--expt-relaxed-constexpr", "--split-compile=0", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default",
+    "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=default",
 ]
 
 

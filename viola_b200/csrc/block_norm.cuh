@@ -1,0 +1,704 @@
+// Kernels of block_norm.cu and their launches; one source file per pair of stream and branch types instantiates them.
+#pragma once
+#include <atomic>
+#include <climits>
+
+#include "api.h"
+#include "common/numerics.cuh"
+
+namespace vb {
+
+constexpr unsigned kAll = 0xffffffffu;
+
+struct NormVector {            // [samples, cols] (or [cols] with pitch 0), null = absent
+  const void* data;
+  int dtype;
+  int wide;                    // rows start on 16-byte boundaries
+  long long pitch;
+};
+struct NormArgs {
+  int rows, cols, tokens;      // tokens: rows of a sample
+  int warps;                   // warps of a row
+  float alpha, eps;
+  const void *x, *y;
+  NormVector weight, gate, next_weight, next_scale;
+  void *out, *h;
+  float *ry, *ru;              // forward: written when not null; backward: read
+  // backward
+  const void *dout, *dh;       // either may be null
+  void *dx, *dy;               // either may be null
+  void *dgate, *dnext_scale;   // gradients of per-sample vectors, or null
+  float* sums;                 // [blocks][2][cols]: column sums of d * yh and of dh * uh for the shared vectors, or null
+  int totals_shared;           // where sums of several samples meet: 1 in shared memory, 0 in `sums` itself (one group to a block)
+  float* parked;               // [row groups][2][2][cols]: the same of samples that another group shares, or null
+  int depth;                   // rows fetched ahead (0: none)
+  int slot_bytes;              // shared memory of one fetched row
+};
+
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ void assign(float& to, float v) { to = v; }
+__device__ __forceinline__ void assign(__nv_bfloat16& to, float v) { to = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void assign(__half& to, float v) { to = __float2half_rn(v); }
+
+// VEC neighbouring values as they are stored
+template <typename T, int VEC> struct Piece {
+  static constexpr int kBytes = VEC * (int)sizeof(T);
+  static constexpr bool kWide = kBytes >= 16;
+  union {
+    T value[VEC];
+    uint4 word[kWide ? kBytes / 16 : 1];
+  };
+  __device__ __forceinline__ Piece() {}
+  __device__ __forceinline__ Piece& operator=(const Piece& other) {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) word[i] = other.word[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) value[i] = other.value[i];
+    }
+    return *this;
+  }
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) word[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) value[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kWide) {
+#pragma unroll
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = word[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) p[i] = value[i];
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) assign(value[i], 0.f);
+  }
+  __device__ __forceinline__ float get(int i) const { return as_float(value[i]); }
+  __device__ __forceinline__ void set(int i, float v) { assign(value[i], v); }
+};
+
+// ---- fetching rows ahead -------------------------------------------------------------------------------------------
+// A thread copies the pieces of the next rows that it will need itself into its own 16-byte places in shared memory
+// (cp.async), so nothing but its own copies has to be waited for: no barrier, and no registers hold the rows in flight.
+__device__ __forceinline__ void copy_ahead(uint32_t to, const void* from, bool through_l1) {
+  if (through_l1) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+  else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait(int pending) {     // all but the youngest `pending` groups have arrived
+  if (pending >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
+  else if (pending == 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else asm volatile("cp.async.wait_group 1;" ::: "memory");
+}
+
+// One tensor's part of a slot: V pieces of VEC values per thread, 16-byte words of neighbouring threads next to each other
+template <typename T, int VEC, int V> struct Strip {
+  static constexpr int kWords = Piece<T, VEC>::kBytes / 16;  // 0: too narrow to be fetched ahead
+  __device__ __forceinline__ static int bytes(int threads) { return V * kWords * threads * 16; }
+  // fp32 pieces are two words apart in memory: the halves of a 32-byte sector meet in L1
+  __device__ __forceinline__ static void fetch(uint32_t slot, const T* row, int tid, int threads, int cols) {
+    if constexpr (kWords > 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * VEC;
+        if (c < cols)
+#pragma unroll
+          for (int w = 0; w < kWords; ++w)
+            copy_ahead(slot + ((j * kWords + w) * threads + tid) * 16, row + c + w * (16 / (int)sizeof(T)), kWords > 1);
+      }
+    }
+  }
+  __device__ __forceinline__ static void take(const unsigned char* slot, int j, int tid, int threads, Piece<T, VEC>& piece) {
+    if constexpr (kWords > 0) {
+#pragma unroll
+      for (int w = 0; w < kWords; ++w)
+        piece.word[w] = *reinterpret_cast<const uint4*>(slot + ((j * kWords + w) * threads + tid) * 16);
+    }
+  }
+};
+
+// Sums N values over the warps of a row; every thread gets them.  `turn` alternates between two buffers, so that one
+// barrier per call is enough: a warp can only reach the buffer's next use through the other buffer's barrier.
+// Rows that a block works on at the same time meet at barriers of their own.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int warps, int group, float (*buffer)[N][32], int& turn) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(kAll, v[n], o);
+  if (warps == 1) return;
+  const int lane = threadIdx.x & 31, first = group * warps;
+  if (lane == 0) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) buffer[turn][n][threadIdx.x >> 5] = v[n];
+  }
+  // (named one by one: a barrier number in a register would reserve all sixteen for the block)
+  if (group == 0) asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
+  else if (group == 1) asm volatile("bar.sync 2, %0;" ::"r"(warps * 32) : "memory");
+  else if (group == 2) asm volatile("bar.sync 3, %0;" ::"r"(warps * 32) : "memory");
+  else asm volatile("bar.sync 4, %0;" ::"r"(warps * 32) : "memory");
+  if (warps <= 4) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      v[n] = buffer[turn][n][first] + buffer[turn][n][first + 1];
+      if (warps > 2) v[n] += buffer[turn][n][first + 2];
+      if (warps > 3) v[n] += buffer[turn][n][first + 3];
+    }
+  } else {
+    // every warp adds the warps' sums for itself: one value a lane, 8, 16 or 32 lanes
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = lane < warps ? buffer[turn][n][first + lane] : 0.f;
+    if (warps > 16)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], 16);
+    if (warps > 8)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], 8);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], o);
+#pragma unroll
+    for (int n = 0; n < N; ++n) v[n] = __shfl_sync(kAll, v[n], 0);
+  }
+  turn ^= 1;
+}
+
+// fp32 values of a thread's columns in shared memory, in places of its own (no barrier): value i of piece j
+template <int VEC>
+__device__ __forceinline__ int own_place(int j, int i, int tid, int threads) {
+  return VEC == 1 ? j * threads + tid : ((j * (VEC / 4) + i / 4) * threads + tid) * 4 + i % 4;
+}
+template <int VEC>
+__device__ __forceinline__ void own_values(const float* area, int j, int tid, int threads, float (&v)[VEC]) {
+  if constexpr (VEC == 1) {
+    v[0] = area[own_place<VEC>(j, 0, tid, threads)];
+  } else {
+#pragma unroll
+    for (int w = 0; w < VEC / 4; ++w) {
+      const float4 f = *reinterpret_cast<const float4*>(area + own_place<VEC>(j, 4 * w, tid, threads));
+      v[4 * w] = f.x; v[4 * w + 1] = f.y; v[4 * w + 2] = f.z; v[4 * w + 3] = f.w;
+    }
+  }
+}
+
+__device__ __forceinline__ float vector_value(const NormVector& v, long long sample, int c, float shift, float otherwise) {
+  return v.data != nullptr ? shift + load_as_float(v.data, sample * v.pitch + c, v.dtype) : otherwise;
+}
+// VEC neighbouring values of an optional vector (absent: 1) plus `shift`
+template <int VEC>
+__device__ __forceinline__ void vector_values(const NormVector& v, long long sample, int c, float shift, float (&f)[VEC]) {
+  if (v.data == nullptr) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+    return;
+  }
+  const long long at = sample * v.pitch + c;
+  if (VEC == 8 && v.wide) {
+    if (v.dtype == kF32) {
+      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(v.data) + at);
+#pragma unroll
+      for (int w = 0; w < VEC / 4; ++w) {
+        const float4 t = p[w];
+        f[4 * w] = t.x; f[4 * w + 1] = t.y; f[4 * w + 2] = t.z; f[4 * w + 3] = t.w;
+      }
+    } else {
+      Piece<__nv_bfloat16, VEC> raw;
+      raw.load(reinterpret_cast<const __nv_bfloat16*>(v.data) + at);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        f[i] = v.dtype == kBF16 ? raw.get(i) : __half2float(__ushort_as_half(__bfloat16_as_ushort(raw.value[i])));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) f[i] = load_as_float(v.data, at + i, v.dtype);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) f[i] += shift;
+}
+
+// product of two optional vectors (the second plus `shift`) for the columns of one thread; once per sample
+template <int VEC, int V>
+__device__ __forceinline__ void store_gain(const NormVector& a, const NormVector& b, float shift, long long sample, int tid,
+                                           int threads, int cols, float* area) {
+#pragma unroll 1
+  for (int j = 0; j < V; ++j) {
+    const int c = (tid + j * threads) * VEC;
+    if (c < cols) {
+      float f[VEC], g[VEC];
+      vector_values<VEC>(a, sample, c, 0.f, f);
+      vector_values<VEC>(b, sample, c, shift, g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) area[own_place<VEC>(j, i, tid, threads)] = f[i] * g[i];
+    }
+  }
+}
+
+// pieces of rows too wide for registers are walked without unrolling
+#define VB_PIECES _Pragma("unroll (V > 4 ? 1 : V)")
+
+template <typename TX, typename TY, int VEC, int V, int THREADS, bool POST, bool PRE>
+__global__ void __launch_bounds__(THREADS)
+norm_forward_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float buffer[2][1][32];
+  using SX = Strip<TX, VEC, V>;
+  using SY = Strip<TY, VEC, V>;
+  const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
+  const int groups = blockDim.x / threads, units = gridDim.x * groups;
+  const int per_unit = (a.rows + units - 1) / units;
+  const long long first = (long long)(blockIdx.x * groups + group) * per_unit;
+  const long long last = min(first + per_unit, (long long)a.rows);
+  const TX* x = reinterpret_cast<const TX*>(a.x);
+  const TY* y = reinterpret_cast<const TY*>(a.y);
+  const float inverse = 1.f / (float)a.cols;
+  const int slots = a.depth + 1, x_bytes = SX::bytes(threads);
+  unsigned char* mine = ring + (size_t)group * slots * a.slot_bytes;
+  auto fetch = [&](long long row, int place) {
+    if (row < last) {
+      const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine + place * a.slot_bytes);
+      SX::fetch(slot, x + row * a.cols, tid, threads, a.cols);
+      if (POST) SY::fetch(slot + x_bytes, y + row * a.cols, tid, threads, a.cols);
+    }
+    copy_commit();
+  };
+  for (int d = 0; d < a.depth; ++d) fetch(first + d, d);
+  float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * V * VEC * threads;
+  float* next_gains = gains + V * VEC * threads;
+  long long sample = first / a.tokens, sample_end = first;
+  int turn = 0, head = 0;
+  for (long long row = first; row < last; ++row) {
+    Piece<TX, VEC> px[V];
+    Piece<TY, VEC> py[V];
+    const long long base = row * a.cols;
+    if (VEC > 1 && a.depth > 0) {
+      const int ahead = head + a.depth;
+      fetch(row + a.depth, ahead >= slots ? ahead - slots : ahead);
+      copy_wait(a.depth);
+      const unsigned char* slot = mine + head * a.slot_bytes;
+      head = head + 1 == slots ? 0 : head + 1;
+VB_PIECES
+      for (int j = 0; j < V; ++j) {
+        SX::take(slot, j, tid, threads, px[j]);
+        if (POST) SY::take(slot + x_bytes, j, tid, threads, py[j]);
+      }
+    } else {
+VB_PIECES
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * VEC;
+        if (c < a.cols) {
+          px[j].load(x + base + c);
+          if (POST) py[j].load(y + base + c);
+        }
+      }
+    }
+    if (row >= sample_end) {
+      if (row > first) ++sample;
+      sample_end = (sample + 1) * a.tokens;
+      if (POST) store_gain<VEC, V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
+      if (PRE) store_gain<VEC, V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
+    }
+    float u[V][VEC], sum[1] = {0.f};
+    if (POST) {
+VB_PIECES
+      for (int j = 0; j < V; ++j)
+        if ((tid + j * threads) * VEC < a.cols)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[0] = fmaf(py[j].get(i), py[j].get(i), sum[0]);
+      row_sum<1>(sum, a.warps, group, buffer, turn);
+      const float ry = rsqrtf(fmaf(sum[0], inverse, a.eps));
+      if (tid == 0 && a.ry != nullptr) a.ry[row] = ry;
+VB_PIECES
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * VEC;
+        if (c < a.cols) {
+          Piece<TX, VEC> o;
+          float gain[VEC];
+          own_values<VEC>(gains, j, tid, threads, gain);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            u[j][i] = fmaf(a.alpha, px[j].get(i), py[j].get(i) * ry * gain[i]);
+            o.set(i, u[j][i]);
+          }
+          o.store(reinterpret_cast<TX*>(a.out) + base + c);
+        }
+      }
+    } else {
+VB_PIECES
+      for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) u[j][i] = px[j].get(i);
+    }
+    if (PRE) {
+      sum[0] = 0.f;
+VB_PIECES
+      for (int j = 0; j < V; ++j)
+        if ((tid + j * threads) * VEC < a.cols)
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) sum[0] = fmaf(u[j][i], u[j][i], sum[0]);
+      row_sum<1>(sum, a.warps, group, buffer, turn);
+      const float ru = rsqrtf(fmaf(sum[0], inverse, a.eps));
+      if (tid == 0 && a.ru != nullptr) a.ru[row] = ru;
+VB_PIECES
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * VEC;
+        if (c < a.cols) {
+          Piece<TY, VEC> o;
+          float gain[VEC];
+          own_values<VEC>(next_gains, j, tid, threads, gain);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) o.set(i, u[j][i] * ru * gain[i]);
+          o.store(reinterpret_cast<TY*>(a.h) + base + c);
+        }
+      }
+    }
+  }
+}
+
+// With q = gate * weight * yh, t = dh * next_weight * (1 + next_scale), uh = u * ru, c = mean(t uh):
+//   d  = dout + ru (t - uh c)                  the gradient of u
+//   dx = alpha d,   dy = ry (d gate weight - yh m),   m = mean(d q)
+// mean(d q) = mean((dout + ru t) q) - ru c mean(uh q), so one reduction of three sums per row serves both norms.
+//
+// Column sums S = sum of d * yh and R = sum of dh * uh give the gradients of the vectors.  Every row group (a block, or
+// part of one where rows are short) takes an equal share of consecutive rows.  With several samples, at the end of one it writes
+// the gradients of the per-sample vectors if it had the whole sample, else parks the sums (place 0: the sample began in
+// an earlier group, 1: it goes on in a later one), and adds them, weighted with the per-sample partner, to the sums of
+// the shared vectors.
+template <typename TX, typename TY, int VEC, int V, int THREADS, bool POST, bool PRE>
+__global__ void __launch_bounds__(THREADS)
+norm_backward_kernel(const NormArgs a) {
+  extern __shared__ __align__(16) unsigned char ring[];
+  __shared__ float buffer[2][3][32];
+  using SX = Strip<TX, VEC, V>;
+  using SY = Strip<TY, VEC, V>;
+  const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
+  const int groups = blockDim.x / threads;
+  const TX* x = reinterpret_cast<const TX*>(a.x);
+  const TY* y = reinterpret_cast<const TY*>(a.y);
+  const TX* dout = reinterpret_cast<const TX*>(a.dout);
+  const TY* dh = reinterpret_cast<const TY*>(a.dh);
+  const float inverse = 1.f / (float)a.cols;
+  const bool samples = a.tokens < a.rows;
+  const long long unit = (long long)blockIdx.x * groups + group, units = min((long long)gridDim.x * groups, (long long)a.rows);
+  const long long first = a.rows * min(unit, units) / units, last = a.rows * min(unit + 1, units) / units;
+  const int slots = a.depth + 1, x_bytes = SX::bytes(threads), y_bytes = SY::bytes(threads);
+  unsigned char* mine = ring + (size_t)group * slots * a.slot_bytes;
+  // dout and, for PRE, x; y for POST; dh for PRE
+  const int at_dout = PRE ? x_bytes : 0, at_y = at_dout + (a.dout != nullptr ? x_bytes : 0), at_dh = at_y + (POST ? y_bytes : 0);
+  int head = 0;
+  auto fetch = [&](long long row, int place) {
+    if (row < last) {
+      const uint32_t slot = (uint32_t)__cvta_generic_to_shared(mine + place * a.slot_bytes);
+      const long long base = row * a.cols;
+      if (PRE) SX::fetch(slot, x + base, tid, threads, a.cols);
+      if (a.dout != nullptr) SX::fetch(slot + at_dout, dout + base, tid, threads, a.cols);
+      if (POST) SY::fetch(slot + at_y, y + base, tid, threads, a.cols);
+      if (PRE) SY::fetch(slot + at_dh, dh + base, tid, threads, a.cols);
+    }
+    copy_commit();
+  };
+  for (int d = 0; d < a.depth; ++d) fetch(first + d, d);
+
+  float post_sum[V][VEC], pre_sum[V][VEC];
+VB_PIECES
+  for (int j = 0; j < V; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) post_sum[j][i] = pre_sum[j][i] = 0.f;
+  // per group: gains, next gains; then, where sums of several samples or groups meet, sums of S and R
+  const int area = V * VEC * threads;
+  float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * area;
+  float* next_gains = gains + area;
+  float* total = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)(groups + group) * 2 * area;
+  if (samples && a.totals_shared) {
+#pragma unroll 1
+    for (int k = 0; k < 2 * V * VEC; ++k) total[k * threads + tid] = 0.f;
+  }
+  const long long first_sample = samples ? first / a.tokens : 0;
+  auto finish_norm = [&](int n, long long sample, const NormVector& weight, const NormVector& partner, float shift, void* grad,
+                         float (&sum)[V][VEC]) {
+    const bool fresh = sample == first_sample, before = sample * a.tokens < first, after = (sample + 1) * a.tokens > last;
+    float* park = a.parked + ((unit * 2 + (before ? 0 : 1)) * 2 + n) * a.cols;
+VB_PIECES
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * VEC;
+      if (c < a.cols) {
+        float f[VEC];
+        if (grad != nullptr) {
+          if (before || after) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) park[c + i] = sum[j][i];
+          } else {
+            vector_values<VEC>(weight, 0, c, 0.f, f);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) store_from_float(grad, sample * a.cols + c + i, partner.dtype, sum[j][i] * f[i]);
+          }
+        }
+        if (a.sums != nullptr) {
+          if (partner.pitch != 0) {
+            vector_values<VEC>(partner, sample, c, shift, f);
+          } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+          }
+          if (a.totals_shared) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) total[n * area + own_place<VEC>(j, i, tid, threads)] += sum[j][i] * f[i];
+          } else {
+            float* to = a.sums + ((long long)blockIdx.x * 2 + n) * a.cols + c;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) to[i] = (fresh ? 0.f : to[i]) + sum[j][i] * f[i];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sum[j][i] = 0.f;
+    }
+  };
+  auto finish_sample = [&](long long sample) {
+    if (POST) finish_norm(0, sample, a.weight, a.gate, 0.f, a.dgate, post_sum);
+    if (PRE) finish_norm(1, sample, a.next_weight, a.next_scale, 1.f, a.dnext_scale, pre_sum);
+  };
+
+  // single values: the next row's are loaded before this row's are worked on
+  constexpr bool kAhead = VEC == 1 && V <= 4;
+  Piece<TX, VEC> next_x[kAhead ? V : 1], next_d[kAhead ? V : 1];
+  Piece<TY, VEC> next_y[kAhead ? V : 1], next_h[kAhead ? V : 1];
+  auto load_next = [&](long long row) {
+    if constexpr (kAhead) {
+      if (row >= last) return;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = tid + j * threads;
+        const long long at = row * a.cols + c;
+        if (a.dout == nullptr) next_d[j].clear();
+        if (c < a.cols) {
+          if (PRE) next_x[j].load(x + at);
+          if (POST) next_y[j].load(y + at);
+          if (a.dout != nullptr) next_d[j].load(dout + at);
+          if (PRE) next_h[j].load(dh + at);
+        }
+      }
+    }
+  };
+  load_next(first);
+  long long sample = first_sample, sample_end = first;
+  int turn = 0;
+  for (long long row = first; row < last; ++row) {
+    const long long base = row * a.cols;
+    Piece<TX, VEC> now_x[kAhead ? V : 1], now_d[kAhead ? V : 1];
+    Piece<TY, VEC> now_y[kAhead ? V : 1], now_h[kAhead ? V : 1];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        now_x[j] = next_x[j];
+        now_d[j] = next_d[j];
+        now_y[j] = next_y[j];
+        now_h[j] = next_h[j];
+      }
+      load_next(row + 1);
+    }
+    const float ry = POST ? a.ry[row] : 0.f, ru = PRE ? a.ru[row] : 0.f;
+    if (row >= sample_end) {
+      if (samples && row > first) finish_sample(sample++);
+      sample_end = samples ? (sample + 1) * a.tokens : last;
+      if (POST) store_gain<VEC, V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
+      if (PRE) store_gain<VEC, V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
+    }
+    const unsigned char* slot = mine + head * a.slot_bytes;
+    if (VEC > 1 && a.depth > 0) {
+      const int ahead = head + a.depth;
+      fetch(row + a.depth, ahead >= slots ? ahead - slots : ahead);
+      copy_wait(a.depth);
+      head = head + 1 == slots ? 0 : head + 1;
+    }
+    float d[V][VEC], yh[V][VEC], uh[V][VEC], sum[3] = {0.f, 0.f, 0.f};
+VB_PIECES
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * VEC;
+      Piece<TX, VEC> px, pd;
+      Piece<TY, VEC> py, ph;
+      float gain[VEC], next_gain[VEC];
+      if (c < a.cols) {
+        if (POST) own_values<VEC>(gains, j, tid, threads, gain);
+        if (PRE) own_values<VEC>(next_gains, j, tid, threads, next_gain);
+        if (a.dout == nullptr) pd.clear();
+        if constexpr (kAhead) {
+          px = now_x[j];
+          pd = now_d[j];
+          py = now_y[j];
+          ph = now_h[j];
+        } else if (VEC > 1 && a.depth > 0) {
+          if (PRE) SX::take(slot, j, tid, threads, px);
+          if (a.dout != nullptr) SX::take(slot + at_dout, j, tid, threads, pd);
+          if (POST) SY::take(slot + at_y, j, tid, threads, py);
+          if (PRE) SY::take(slot + at_dh, j, tid, threads, ph);
+        } else {
+          if (PRE) px.load(x + base + c);
+          if (POST) py.load(y + base + c);
+          if (a.dout != nullptr) pd.load(dout + base + c);
+          if (PRE) ph.load(dh + base + c);
+        }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float q = 0.f, u;
+          d[j][i] = pd.get(i);
+          if (POST) {
+            yh[j][i] = py.get(i) * ry;
+            q = yh[j][i] * gain[i];
+          }
+          if (PRE) {
+            u = POST ? fmaf(a.alpha, px.get(i), q) : px.get(i);
+            uh[j][i] = u * ru;
+            const float g = ph.get(i), t = g * next_gain[i];
+            pre_sum[j][i] = fmaf(g, uh[j][i], pre_sum[j][i]);
+            sum[0] = fmaf(t, uh[j][i], sum[0]);
+            d[j][i] = fmaf(ru, t, d[j][i]);
+            if (POST) sum[2] = fmaf(uh[j][i], q, sum[2]);
+          }
+          if (POST) sum[1] = fmaf(d[j][i], q, sum[1]);
+        }
+      }
+    }
+    row_sum<3>(sum, a.warps, group, buffer, turn);
+    const float pull = ru * sum[0] * inverse;                       // ru c
+    const float m = POST ? (PRE ? fmaf(-pull, sum[2], sum[1]) : sum[1]) * inverse : 0.f;
+VB_PIECES
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * VEC;
+      if (c < a.cols) {
+        Piece<TX, VEC> ox;
+        Piece<TY, VEC> oy;
+        float gain[VEC];
+        if (POST) own_values<VEC>(gains, j, tid, threads, gain);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float whole = PRE ? fmaf(-pull, uh[j][i], d[j][i]) : d[j][i];
+          ox.set(i, POST ? a.alpha * whole : whole);
+          if (POST) {
+            oy.set(i, ry * fmaf(-m, yh[j][i], whole * gain[i]));
+            post_sum[j][i] = fmaf(whole, yh[j][i], post_sum[j][i]);
+          }
+        }
+        if (a.dx != nullptr) ox.store(reinterpret_cast<TX*>(a.dx) + base + c);
+        if (POST && a.dy != nullptr) oy.store(reinterpret_cast<TY*>(a.dy) + base + c);
+      }
+    }
+  }
+  if (samples && first < last) finish_sample(sample);
+  if (a.sums == nullptr || (samples && !a.totals_shared)) return;
+  float* to = a.sums + (long long)blockIdx.x * 2 * a.cols;
+  if (!samples && groups == 1) {
+VB_PIECES
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * VEC;
+      if (c < a.cols)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          to[c + i] = POST ? post_sum[j][i] : 0.f;
+          to[a.cols + c + i] = PRE ? pre_sum[j][i] : 0.f;
+        }
+    }
+    return;
+  }
+  if (!samples) {
+VB_PIECES
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        total[own_place<VEC>(j, i, tid, threads)] = POST ? post_sum[j][i] : 0.f;
+        total[area + own_place<VEC>(j, i, tid, threads)] = PRE ? pre_sum[j][i] : 0.f;
+      }
+  }
+  __syncthreads();
+  // the first group adds the groups' sums in order
+  if (group == 0) {
+#pragma unroll 1
+    for (int k = 0; k < 2 * V * VEC; ++k) {
+      const int n = k / (V * VEC), j = k / VEC % V, i = k % VEC, c = (tid + j * threads) * VEC + i;
+      if (c < a.cols) {
+        const float* from = total + n * area + own_place<VEC>(j, i, tid, threads);
+        float s = from[0];
+        for (int g = 1; g < groups; ++g) s += from[(size_t)g * 2 * area];
+        to[n * a.cols + c] = s;
+      }
+    }
+  }
+}
+
+constexpr int kSharedPerBlock = 227 * 1024;
+
+struct NormShape {
+  int vec, v, warps, groups;   // values per access, accesses per thread, warps per row, rows a block works on at a time
+  int bound;                   // threads that the kernel's template is built for
+  int threads() const { return warps * groups * 32; }
+};
+
+// lets a kernel use as much dynamic shared memory as its launch asks for, once per device
+template <auto Kernel>
+void allow_shared() {
+  static std::atomic<unsigned long long> done{0};
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return;
+  const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return;
+  // what the kernel has statically comes off the limit: two row-sum buffers
+  cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerBlock - 1024);
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
+struct NormLaunch {
+  bool backward, post, pre;
+  int blocks, threads;
+  size_t smem;
+  cudaStream_t stream;
+};
+
+template <auto Kernel>
+void launch_kernel(const NormArgs& a, const NormLaunch& l) {
+  if (l.smem > 48 * 1024 - 1024) allow_shared<Kernel>();
+  Kernel<<<l.blocks, l.threads, l.smem, l.stream>>>(a);
+}
+
+template <bool BACKWARD, typename TX, typename TY, int VEC, int V, int THREADS>
+void launch_norms(const NormArgs& a, const NormLaunch& l) {
+  if constexpr (BACKWARD) {
+    if (l.post && l.pre) launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, true, true>>(a, l);
+    else if (l.post) launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, true, false>>(a, l);
+    else launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, false, true>>(a, l);
+  } else {
+    if (l.post && l.pre) launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, true, true>>(a, l);
+    else if (l.post) launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, true, false>>(a, l);
+    else launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, false, true>>(a, l);
+  }
+}
+
+template <typename TX, typename TY>
+void launch_shape(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
+  if (s.vec == 1) {
+    if (l.backward) s.v == 4 ? launch_norms<true, TX, TY, 1, 4, 256>(a, l) : launch_norms<true, TX, TY, 1, 16, 1024>(a, l);
+    else s.v == 4 ? launch_norms<false, TX, TY, 1, 4, 256>(a, l) : launch_norms<false, TX, TY, 1, 16, 1024>(a, l);
+  } else if (l.backward) {
+    if (s.v == 1) launch_norms<true, TX, TY, 8, 1, 512>(a, l);
+    else if (s.v == 2) launch_norms<true, TX, TY, 8, 2, 512>(a, l);
+    else launch_norms<true, TX, TY, 8, 4, 512>(a, l);
+  } else {
+    if (s.v == 1) launch_norms<false, TX, TY, 8, 1, 256>(a, l);
+    else if (s.v == 2) launch_norms<false, TX, TY, 8, 2, 256>(a, l);
+    else if (s.v == 3) launch_norms<false, TX, TY, 8, 3, 256>(a, l);
+    else if (s.bound == 256) launch_norms<false, TX, TY, 8, 4, 256>(a, l);
+    else launch_norms<false, TX, TY, 8, 4, 512>(a, l);
+  }
+}
+
+}  // namespace vb

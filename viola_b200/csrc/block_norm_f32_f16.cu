@@ -1,0 +1,6 @@
+// Norms around a block: float stream, __half branch.
+#include "block_norm.cuh"
+
+namespace vb {
+template void launch_shape<float, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
+}  // namespace vb
