@@ -575,3 +575,67 @@ def test_operands_on_two_devices_are_refused():
                 lambda: nn.rms_norm_residual(x, other), lambda: nn.rms_norm_modulate(x, other[0])):
         with pytest.raises(ValueError):
             bad()
+
+
+# ------------------------------------------------------------------------------------------------- with the expert linear
+@pytest.mark.parametrize("scaling", ["current", "grouped"])
+def test_expert_linear_leaves_zeros_behind_the_last_expert(scaling, device):
+    layer = nn.GroupedLinear(3, 128, 256, scaling=scaling).to(device)
+    offsets = torch.tensor([0, 5, 5, 140], dtype=torch.int32, device=device)
+    x = randn(0, 300, 128, dtype=BF16).to(device).requires_grad_(True)
+    dirt = torch.full((300, 256), math.nan, dtype=BF16, device=device)       # what the allocator may hand out again
+    del dirt
+    y = layer(x, offsets)
+    assert y[140:].eq(0).all() and y[:140].isfinite().all() and y[:140].ne(0).any()
+    y.backward(torch.ones_like(y))
+    assert x.grad[140:].eq(0).all() and x.grad[:140].ne(0).any()
+
+
+def expert_block(x, logits, mask, first, second, weights, gate):
+    """A block as a model has it: norm, experts, norm, gated residual, norm of the next block."""
+    h = nn.rms_norm_modulate(x, weights[0])
+    routing = nn.route_tokens(logits, 2, mask=mask)
+    plan = nn.plan_experts(routing.indices, first.num_experts)
+    rows = first(nn.dispatch_tokens(h, plan), plan.offsets)
+    rows = second(torch.nn.functional.silu(rows), plan.offsets)
+    y = nn.combine_tokens(rows, routing.weights, plan)
+    out, following = nn.rms_norm_residual(x, y, weights[1], gate, residual_scale=0.9, next_norm=True, next_weight=weights[2])
+    return out, following, routing
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scaling", ["current", "grouped"])
+@pytest.mark.parametrize("padded", [False, True])
+def test_expert_block_matches_the_cpu_path(scaling, padded):
+    """The operators together around FP8 expert linears, kernels against restatements.  Both sides quantise the same values
+    up to rounding; a value on the border of two FP8 codes may fall on either side of it (a step of 2^-3 at most, for a
+    share of about 2^-8 of the values), hence 2 % in the norm."""
+    batch, tokens, width, hidden, experts = 2, 75, 128, 256, 5
+    torch.manual_seed(0)
+    first, second = nn.GroupedLinear(experts, width, hidden, scaling=scaling), nn.GroupedLinear(experts, hidden, width, scaling=scaling)
+    mask = torch.rand(batch, tokens) < 0.7 if padded else None
+    x, logits = torch.randn(batch, tokens, width).bfloat16(), torch.randn(batch, tokens, experts)
+    if padded:
+        logits[~mask] = math.nan
+    weights, gate = [1 + 0.1 * torch.randn(width) for _ in range(3)], torch.randn(batch, width).bfloat16()
+    grads = torch.randn(2, batch, tokens, width).bfloat16()
+    results = []
+    for device in ("cpu", "cuda"):
+        a, b = first.to(device), second.to(device)
+        a.zero_grad()
+        b.zero_grad()
+        leaves = [t.detach().to(device).requires_grad_(True) for t in (x, logits, *weights, gate)]
+        # leave NaN in freed memory, which results that are not written would show
+        dirt = [torch.full((4 * batch * tokens, hidden), math.nan, device=device) for _ in range(4)]
+        del dirt
+        out, following, routing = expert_block(leaves[0], leaves[1], None if mask is None else mask.to(device), a, b, leaves[2:5],
+                                               leaves[5])
+        loss = (out * grads[0].to(device)).float().sum() + (following * grads[1].to(device)).float().sum()
+        (loss + 0.1 * routing.balance_loss + 0.01 * routing.z_loss).backward()
+        results.append([t.detach().float().cpu() for t in (out, following, *(t.grad for t in leaves), a.weight.grad, b.weight.grad)])
+        if padded:
+            assert leaves[1].grad[~mask.to(device)].eq(0).all()
+            torch.testing.assert_close(out[~mask.to(device)], 0.9 * leaves[0][~mask.to(device)], rtol=2 ** -7, atol=0)
+    for i, (cpu, gpu) in enumerate(zip(*results)):
+        assert gpu.isfinite().all(), i
+        assert (gpu - cpu).norm() <= 0.02 * cpu.norm(), (i, float((gpu - cpu).norm() / cpu.norm()))

@@ -64,7 +64,8 @@ typedef struct VbGemmDesc {
                                 // VB_EPI_ACT_BWD: [M, N] activation slope act'(z) saved by the forward pass,
                                 // out = round(acc) * aux
   unsigned int* amax_out;       // VB_EPI_ACT_BWD: atomicMax of |out| as float bits (caller zero-initialises)
-  // expert GEMM: rows of A are grouped by expert; offsets[e]..offsets[e+1] (device, int32, E+1)
+  // expert GEMM: rows of A are grouped by expert; offsets[e]..offsets[e+1] (device, int32, E+1); rows of the result from
+  // offsets[E] on are zeroed
   const int* expert_offsets; int num_experts;
   int* tile_map;         // workspace int32[3 * (ceil(M/128) + E)] when expert_offsets != null
   int* status;           // int32[8] device status word (zeroed by caller) or null

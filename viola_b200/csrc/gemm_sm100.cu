@@ -1198,10 +1198,25 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   }
 }
 
-// Builds the tile -> (row0, row_end, expert) map for the expert GEMM from device offsets.
+// Builds the tile -> (row0, row_end, expert) map for the expert GEMM from device offsets (block 0) and zeroes the rows of
+// the result that no expert has (the other blocks): rows behind the last expert's, which a quantiser with one scale for
+// the whole buffer would otherwise read as they happen to be.
 __global__ void expert_tile_map_kernel(const int* __restrict__ offsets, int num_experts, int max_tiles,
-                                       int* __restrict__ tile_map) {
-  if (threadIdx.x != 0 || blockIdx.x != 0) return;
+                                       int* __restrict__ tile_map, void* __restrict__ out, int rows, long long row_bytes,
+                                       long long pitch_bytes) {
+  if (blockIdx.x > 0) {
+    const bool wide = ((row_bytes | pitch_bytes | (long long)reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    for (long long r = (long long)max(offsets[num_experts], 0) + blockIdx.x - 1; r < rows; r += gridDim.x - 1) {
+      char* row = reinterpret_cast<char*>(out) + r * pitch_bytes;
+      if (wide) {
+        for (long long i = threadIdx.x; i < row_bytes / 16; i += blockDim.x) reinterpret_cast<uint4*>(row)[i] = make_uint4(0, 0, 0, 0);
+      } else {
+        for (long long i = threadIdx.x; i < row_bytes / 2; i += blockDim.x) reinterpret_cast<uint16_t*>(row)[i] = 0;
+      }
+    }
+    return;
+  }
+  if (threadIdx.x != 0) return;
   int t = 0;
   for (int e = 0; e < num_experts; ++e) {
     const int begin = offsets[e], end = offsets[e + 1];
@@ -1477,7 +1492,9 @@ static int launch(const VbGemmDesc& d, cudaStream_t stream, int split = 1) {
     }
   }
   if (expert) {
-    expert_tile_map_kernel<<<1, 32, 0, stream>>>(d.expert_offsets, d.num_experts, a.num_m_tiles, d.tile_map);
+    const long long size = d.out_dtype == 0 ? 4 : 2;
+    expert_tile_map_kernel<<<1 + 64, 128, 0, stream>>>(d.expert_offsets, d.num_experts, a.num_m_tiles, d.tile_map, d.out, d.M,
+                                                       d.N * size, d.ldo * size);
   }
   a.split_k = 1;
   a.kb_per_split = a.num_k_blocks;

@@ -613,10 +613,11 @@ def gated_backward(gu, dh, activation):
 
 # ------------------------------------------------------------------------------ expert (ragged-M) GEMM
 def expert_gemm(a, w, offsets, sa, sw, *, out_dtype, group=None, sa_kmajor=False, sw_kmajor=False, out=None):
-    """out[rows of expert e] = A[rows of e] . W[e]^T.  ``w`` is [E, N, K]; ``offsets`` int32 [E+1] on device."""
+    """out[rows of expert e] = A[rows of e] . W[e]^T.  ``w`` is [E, N, K]; ``offsets`` int32 [E+1] on device.  Rows that no
+    expert has (from ``offsets[E]`` on) come out as zero."""
     experts, n, k = w.shape
     if not a.is_cuda:
-        result = torch.empty((a.shape[0], n), dtype=out_dtype)
+        result = torch.zeros((a.shape[0], n), dtype=out_dtype)
         bounds = offsets.tolist()
         for e in range(experts):
             lo, hi = bounds[e], bounds[e + 1]
