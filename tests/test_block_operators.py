@@ -639,3 +639,157 @@ def test_expert_block_matches_the_cpu_path(scaling, padded):
     for i, (cpu, gpu) in enumerate(zip(*results)):
         assert gpu.isfinite().all(), i
         assert (gpu - cpu).norm() <= 0.02 * cpu.norm(), (i, float((gpu - cpu).norm() / cpu.norm()))
+
+
+# ---------------------------------------------------------------------------------------------- graphs, streams, large sizes
+def whole_pass(logits, x, y, weights, gate, mask):
+    """Every operator forward and backward; leaves in, results and gradients out."""
+    routing = nn.route_tokens(logits, 3, mask=mask)
+    plan = nn.plan_experts(routing.indices, logits.shape[-1])
+    rows = nn.dispatch_tokens(x, plan)
+    z = nn.combine_tokens(rows * 1.5, routing.weights, plan).view(x.shape)
+    out, h = nn.rms_norm_residual(y, z, weights, gate, next_norm=True, next_weight=weights)
+    loss = out.sum() + (h * h).sum() + 0.1 * routing.balance_loss + 0.01 * routing.z_loss
+    return [routing.indices, plan.offsets, plan.positions, rows.detach(), out.detach(), h.detach(),
+            *torch.autograd.grad(loss, (logits, x, y, weights, gate))]
+
+
+def pass_leaves(seed, batch=4, tokens=300, width=192, experts=40):
+    return [randn(seed, batch * tokens, experts).cuda().requires_grad_(True),
+            *(randn(seed + i, batch, tokens, width).cuda().requires_grad_(True) for i in (1, 2)),
+            randn(seed + 3, width).cuda().requires_grad_(True), randn(seed + 4, batch, width).cuda().requires_grad_(True),
+            (torch.rand(batch * tokens, generator=torch.Generator().manual_seed(seed)) < 0.8).cuda()]
+
+
+@pytest.mark.gpu
+def test_results_repeat_bit_for_bit():
+    leaves = pass_leaves(0, batch=16, tokens=1000)
+    first = whole_pass(*leaves)
+    for _ in range(3):
+        for a, b in zip(first, whole_pass(*leaves)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_graphs_share_nothing():
+    """Two captured passes, replayed on new inputs, one after the other and on two streams at once."""
+    torch.cuda.synchronize()
+    captured = []
+    for seed in (0, 50):
+        leaves = pass_leaves(seed)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            whole_pass(*leaves)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            results = whole_pass(*leaves)
+        captured.append((graph, leaves, results))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for attempt in range(5):
+        expected = []
+        for i, (_, leaves, _) in enumerate(captured):
+            fresh = pass_leaves(1000 + 100 * attempt + 10 * i)
+            for leaf, value in zip(leaves, fresh):
+                leaf.detach().copy_(value.detach())
+            expected.append([t.clone() for t in whole_pass(*fresh)])
+        torch.cuda.synchronize()
+        for stream, (graph, _, _) in zip(streams, captured):
+            with torch.cuda.stream(stream):
+                for _ in range(3):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for wanted, (_, _, results) in zip(expected, captured):
+            for a, b in zip(wanted, results):
+                assert torch.equal(a, b)
+    captured.clear()
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    sets = [pass_leaves(7), pass_leaves(70)]
+    expected = [whole_pass(*leaves) for leaves in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for stream, leaves, results in zip(streams, sets, got):
+            with torch.cuda.stream(stream):
+                results.append(whole_pass(*leaves))
+    torch.cuda.synchronize()
+    for wanted, results in zip(expected, got):
+        for result in results:
+            for a, b in zip(wanted, result):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    logits, x, y, weights, gate, mask = pass_leaves(3)
+    out = nn.rms_norm_modulate(x, weights)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+@pytest.mark.gpu
+def test_in_place_changes_of_saved_inputs_are_noticed():
+    logits, x, y, weights, gate, mask = pass_leaves(4)
+    values = x * 1.0
+    out = nn.rms_norm_residual(values, y, weights, gate, next_norm=True)[1]
+    values.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Buffers of more than 2^31 values: the last rows against the same rows alone."""
+    tokens, top_k, width, last = 131200, 8, 2056, 37
+    x = torch.randn(tokens, width, device="cuda", dtype=BF16)
+    indices = torch.arange(top_k, device="cuda", dtype=torch.int32).repeat(tokens, 1)
+    plan = nn.plan_experts(indices, top_k)
+    assert tokens * top_k * width > 2 ** 31
+    rows = nn.dispatch_tokens(x, plan)
+    for e in (0, top_k - 1):
+        assert torch.equal(rows[(e + 1) * tokens - last:(e + 1) * tokens], x[-last:])
+    weights = torch.rand(tokens, top_k, device="cuda")
+    small = nn.plan_experts(indices[:last], top_k)
+    dout = torch.randn(tokens, width, device="cuda", dtype=BF16)
+    rows, weights = rows.requires_grad_(True), weights.requires_grad_(True)
+    out = nn.combine_tokens(rows, weights, plan)
+    drows, dweights = torch.autograd.grad(out, (rows, weights), dout)
+    tail = [t.detach().requires_grad_(True) for t in (nn.dispatch_tokens(x[-last:], small), weights[-last:])]
+    tail_out = nn.combine_tokens(*tail, small)
+    tail_grads = torch.autograd.grad(tail_out, tail, dout[-last:])
+    assert torch.equal(out[-last:], tail_out)
+    # few tokens are shared out to more warps each: two orders of the same sum, each off by at most n u * sum of |terms|
+    terms = (dout[-last:].float().abs() * x[-last:].float().abs()).sum(1, keepdim=True)
+    assert ((dweights[-last:] - tail_grads[1]).abs() <= 2 * width * 2.0 ** -24 * terms).all()
+    assert torch.equal(drows[-last:], tail_grads[0][-last:])
+    del rows, drows, out, x, dout, weights
+    rows, width = 262200, 8200
+    assert rows * width > 2 ** 31
+    x = torch.randn(1, rows, width, device="cuda", dtype=BF16).requires_grad_(True)
+    h = nn.rms_norm_modulate(x)
+    dx, = torch.autograd.grad(h, x, h.detach())
+    part = x.detach()[:, -last:].clone().requires_grad_(True)
+    h_part = nn.rms_norm_modulate(part)
+    assert torch.equal(h[:, -last:], h_part)
+    assert torch.equal(dx[:, -last:], torch.autograd.grad(h_part, part, h_part.detach())[0])
+    del x, h, dx
+    tokens, experts = 2100000, 1024
+    assert tokens * experts > 2 ** 31
+    logits = torch.randn(tokens, experts, device="cuda", dtype=BF16)
+    out, part = nn.route_tokens(logits, 2), nn.route_tokens(logits[-last:], 2)
+    assert torch.equal(out.indices[-last:], part.indices) and torch.equal(out.weights[-last:], part.weights)
+    assert int(out.counts.sum()) == 2 * tokens
+
+
+@pytest.mark.gpu
+def test_another_device_than_the_current_one():
+    if torch.cuda.device_count() < 2:
+        pytest.skip("one GPU")
+    leaves = [t.detach().to("cuda:1").requires_grad_(t.requires_grad) for t in pass_leaves(11)]
+    expected = whole_pass(*pass_leaves(11))
+    for a, b in zip(expected, whole_pass(*leaves)):
+        assert b.device.index == 1 and torch.equal(a.cpu(), b.cpu())
