@@ -591,6 +591,17 @@ def test_expert_linear_leaves_zeros_behind_the_last_expert(scaling, device):
     assert x.grad[140:].eq(0).all() and x.grad[:140].ne(0).any()
 
 
+def test_expert_gemm_leaves_the_rest_of_a_given_result(device):
+    codes, weights = randn(1, 40, 128).to(device), randn(2, 2, 64, 128).to(device)
+    scale, offsets = torch.ones(1, device=device), torch.tensor([0, 7, 25], dtype=torch.int32, device=device)
+    q, _ = ops.quantize(codes, scale)
+    w, _ = ops.quantize(weights.view(128, 128), scale)
+    out = torch.full((40, 64), 7.0, device=device)
+    assert ops.expert_gemm(q, w.view(2, 64, 128), offsets, scale, scale, out_dtype=FP32, out=out) is out
+    fresh = ops.expert_gemm(q, w.view(2, 64, 128), offsets, scale, scale, out_dtype=FP32)
+    assert out[25:].eq(7).all() and fresh[25:].eq(0).all() and torch.equal(out[:25], fresh[:25])
+
+
 def expert_block(x, logits, mask, first, second, weights, gate):
     """A block as a model has it: norm, experts, norm, gated residual, norm of the next block."""
     h = nn.rms_norm_modulate(x, weights[0])

@@ -64,9 +64,9 @@ typedef struct VbGemmDesc {
                                 // VB_EPI_ACT_BWD: [M, N] activation slope act'(z) saved by the forward pass,
                                 // out = round(acc) * aux
   unsigned int* amax_out;       // VB_EPI_ACT_BWD: atomicMax of |out| as float bits (caller zero-initialises)
-  // expert GEMM: rows of A are grouped by expert; offsets[e]..offsets[e+1] (device, int32, E+1); rows of the result from
-  // offsets[E] on are zeroed
+  // expert GEMM: rows of A are grouped by expert; offsets[e]..offsets[e+1] (device, int32, E+1)
   const int* expert_offsets; int num_experts;
+  int clear_tail;        // expert GEMM: 1 = zero the rows of `out` from offsets[E] on, 0 = leave them as they are
   int* tile_map;         // workspace int32[3 * (ceil(M/128) + E)] when expert_offsets != null
   int* status;           // int32[8] device status word (zeroed by caller) or null
   int force_bn;          // 0 = auto, else 64 / 128 / 256

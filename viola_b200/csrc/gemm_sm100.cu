@@ -1198,9 +1198,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   }
 }
 
-// Builds the tile -> (row0, row_end, expert) map for the expert GEMM from device offsets (block 0) and zeroes the rows of
-// the result that no expert has (the other blocks): rows behind the last expert's, which a quantiser with one scale for
-// the whole buffer would otherwise read as they happen to be.
+// Builds the tile -> (row0, row_end, expert) map for the expert GEMM from device offsets (block 0) and, in the other blocks if
+// there are any, zeroes the rows of the result behind the last expert's, which a quantiser with one scale for the whole
+// buffer would otherwise read as they happen to be.
 __global__ void expert_tile_map_kernel(const int* __restrict__ offsets, int num_experts, int max_tiles,
                                        int* __restrict__ tile_map, void* __restrict__ out, int rows, long long row_bytes,
                                        long long pitch_bytes) {
@@ -1493,7 +1493,7 @@ static int launch(const VbGemmDesc& d, cudaStream_t stream, int split = 1) {
   }
   if (expert) {
     const long long size = d.out_dtype == 0 ? 4 : 2;
-    expert_tile_map_kernel<<<1 + 64, 128, 0, stream>>>(d.expert_offsets, d.num_experts, a.num_m_tiles, d.tile_map, d.out, d.M,
+    expert_tile_map_kernel<<<d.clear_tail ? 1 + 64 : 1, 128, 0, stream>>>(d.expert_offsets, d.num_experts, a.num_m_tiles, d.tile_map, d.out, d.M,
                                                        d.N * size, d.ldo * size);
   }
   a.split_k = 1;

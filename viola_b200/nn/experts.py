@@ -22,6 +22,7 @@ import torch
 from .. import ops
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_MAX_WIDTH = 1 << 22
 
 
 class Routing(NamedTuple):
@@ -113,7 +114,7 @@ def dispatch_tokens(x, plan):
     offsets, positions = _check_plan(plan, x, "x")
     _float(x, "x")
     width = x.shape[-1]
-    if width < 1 or x.numel() != positions.shape[0] * width:
+    if not 1 <= width <= _MAX_WIDTH or x.numel() != positions.shape[0] * width:
         raise ValueError(f"x of shape {tuple(x.shape)} does not hold the plan's {positions.shape[0]} tokens")
     return ops.expert_dispatch(x, positions, offsets)
 
@@ -129,7 +130,7 @@ def combine_tokens(rows, weights, plan):
     _float(weights, "weights")
     _same_device(weights, "weights", rows)
     tokens, top_k = positions.shape
-    if rows.dim() != 2 or rows.shape[0] != tokens * top_k or rows.shape[1] < 1:
+    if rows.dim() != 2 or rows.shape[0] != tokens * top_k or not 1 <= rows.shape[1] <= _MAX_WIDTH:
         raise ValueError(f"rows must be [{tokens * top_k}, width], got {tuple(rows.shape)}")
     if weights.dim() < 1 or weights.shape[-1] != top_k or weights.numel() != tokens * top_k:
         raise ValueError(f"weights of shape {tuple(weights.shape)} do not match the plan's {tokens} tokens x {top_k} choices")

@@ -285,7 +285,7 @@ def _check_mn(t):
 
 def _gemm(a, b, out, epilogue, n_logical, *, sa=None, sb=None, layout=_NO_GROUP, bias=None, alpha=1.0, beta=0.0,
           resid=None, out_t=None, symmetric=False, activation=0, aux=None, expert_offsets=None, tile_map=None,
-          force_bn=0, batch=1, a_mn=False, b_mn=False, amax_out=None, force_split=0, accumulate=False):
+          force_bn=0, batch=1, a_mn=False, b_mn=False, amax_out=None, force_split=0, accumulate=False, clear_tail=False):
     multiple = 16 if a.element_size() == 1 else 8
     a = _check_mn(a) if a_mn else _pad_k(a, multiple)
     b = _check_mn(b) if b_mn else _pad_k(b, multiple)
@@ -295,7 +295,7 @@ def _gemm(a, b, out, epilogue, n_logical, *, sa=None, sb=None, layout=_NO_GROUP,
         _ops().gemm(a, b, out, epilogue, n_logical, sa, sb, list(layout), bias, float(alpha), float(beta), resid, out_t,
                     bool(symmetric), int(activation), aux, expert_offsets, tile_map, status,
                     int(tile) | (int(force_split) << 16), int(batch),
-                    bool(a_mn), bool(b_mn), amax_out, bool(accumulate))
+                    bool(a_mn), bool(b_mn), amax_out, bool(accumulate), bool(clear_tail))
 
     if not force_bn and not accumulate and (tuning._enabled or tuning._choices):
         # the output-tile width of this shape: recorded choice, or (tuning on) measured now on these operands
@@ -613,8 +613,8 @@ def gated_backward(gu, dh, activation):
 
 # ------------------------------------------------------------------------------ expert (ragged-M) GEMM
 def expert_gemm(a, w, offsets, sa, sw, *, out_dtype, group=None, sa_kmajor=False, sw_kmajor=False, out=None):
-    """out[rows of expert e] = A[rows of e] . W[e]^T.  ``w`` is [E, N, K]; ``offsets`` int32 [E+1] on device.  Rows that no
-    expert has (from ``offsets[E]`` on) come out as zero."""
+    """out[rows of expert e] = A[rows of e] . W[e]^T.  ``w`` is [E, N, K]; ``offsets`` int32 [E+1] on device.  Rows
+    behind the last expert's (from ``offsets[E]`` on) are zero in a new result and left as they are in ``out``."""
     experts, n, k = w.shape
     if not a.is_cuda:
         result = torch.zeros((a.shape[0], n), dtype=out_dtype)
@@ -630,7 +630,11 @@ def expert_gemm(a, w, offsets, sa, sw, *, out_dtype, group=None, sa_kmajor=False
                 sw_e = sw_all.reshape(experts, -1, sw_all.shape[-1])[e]
                 result[lo:hi] = reference.group_gemm(a[lo:hi], w[e], sa_e, sw_e, group[0], group[1],
                                                      out_dtype=out_dtype)
-        return result if out is None else out.copy_(result)
+        if out is None:
+            return result
+        out[:bounds[-1]] = result[:bounds[-1]]
+        return out
+    clear_tail = out is None
     if out is None:
         out = torch.empty((a.shape[0], n), device=a.device, dtype=out_dtype)
     tile_map = torch.empty(3 * ((a.shape[0] + 127) // 128 + experts), device=a.device, dtype=torch.int32)
@@ -640,7 +644,8 @@ def expert_gemm(a, w, offsets, sa, sw, *, out_dtype, group=None, sa_kmajor=False
         layout = _group_layout(a, experts * n, k, group[0], group[1], sa_kmajor, sw_kmajor)
         assert layout is not None and n % group[1][0] == 0, "expert GEMM needs 1xK activation groups and N % block == 0"
         sw = sw.reshape(-1, sw.shape[-1]) if not sw_kmajor else sw
-    return _gemm(a, w2, out, EPI_LINEAR, n, sa=sa, sb=sw, layout=layout, expert_offsets=offsets, tile_map=tile_map)
+    return _gemm(a, w2, out, EPI_LINEAR, n, sa=sa, sb=sw, layout=layout, expert_offsets=offsets, tile_map=tile_map,
+                 clear_tail=clear_tail)
 
 
 # ------------------------------------------------------------------------------ Newton-Schulz GEMM
