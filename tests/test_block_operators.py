@@ -494,6 +494,63 @@ def test_norm_strides_views_and_broadcast_vectors(device):
     assert per_row.shape == (batch * tokens, width)
 
 
+@pytest.mark.parametrize("width", [40, 250, 263, 1153])
+@pytest.mark.parametrize("types", [(FP32, BF16), (FP16, FP16)])
+def test_norm_rows_at_any_address(width, types, device):
+    """Contiguous streams that begin anywhere in their storage, results and gradients included, next to untouched memory."""
+    stream, branch = types
+    for offset in (1, 2, 3, 6, 7):
+        case = (2, 3, width, stream, branch, True, "sample", "sample", True, True, 0.75)
+        v, dout, dh = norm_inputs(case, offset)
+        expected = oracle.block_norm(**v, residual_scale=0.75, dout=dout, dh=dh)
+
+        def moved(t):
+            store = torch.full((t.numel() + 16,), math.nan, dtype=t.dtype, device=device)
+            view = store[offset:offset + t.numel()].view(t.shape)
+            view.copy_(t)
+            return view
+
+        leaves = {n: moved(t).requires_grad_(True) if n in ("x", "y") else t.to(device).requires_grad_(True) for n, t in v.items()}
+        out, h = call_norm(case, leaves)
+        torch.autograd.backward([out, h], [moved(dout), moved(dh)])
+        for name, t in (("out", out), ("h", h)):
+            oracle.assert_matches(t, expected[name], width, name)
+        for name, leaf in leaves.items():
+            oracle.assert_matches(leaf.grad, expected["d" + name], width + 6, "d" + name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [8, 9, 24, 257, 519, 1031])
+@pytest.mark.parametrize("dtype", [FP32, BF16])
+def test_norm_writes_its_rows_and_nothing_else(cols, dtype):
+    """The C entry writes results at odd addresses: the bytes around them stay."""
+    import ctypes
+
+    class Vector(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int), ("pitch", ctypes.c_longlong)]
+
+    class Norm(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols", "tokens", "x_dtype", "y_dtype")] + [
+            ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float), ("x", ctypes.c_void_p), ("y", ctypes.c_void_p)] + [
+            (n, Vector) for n in ("weight", "gate", "next_weight", "next_scale")] + [
+            (n, ctypes.c_void_p) for n in ("out", "h", "ry", "ru")]
+
+    ops.load()
+    library = ctypes.CDLL(str(ops._LIB_PATH))
+    rows, code = 5, {FP32: 0, BF16: 1}[dtype]
+    x, y = randn(0, rows, cols, dtype=dtype).cuda(), randn(1, rows, cols, dtype=dtype).cuda()
+    expected, following = nn.rms_norm_residual(x, y, next_norm=True)
+    for offset in range(8):
+        stores = [torch.full((rows * cols + 32,), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+        views = [s[8 + offset:8 + offset + rows * cols] for s in stores]
+        norm = Norm(rows, cols, rows, code, code, 1.0, 1e-6, x.data_ptr(), y.data_ptr(), *[Vector(None, 0, 0)] * 4,
+                    views[0].data_ptr(), views[1].data_ptr(), None, None)
+        assert library.vb_block_norm(ctypes.byref(norm), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        for store, view, wanted in zip(stores, views, (expected, following)):
+            assert torch.equal(view.view(rows, cols), wanted)
+            assert store[:8 + offset].eq(7).all() and store[8 + offset + rows * cols:].eq(7).all()
+
+
 def test_norm_gradient_of_an_expanded_gate(device):
     """A gate broadcast over the batch outside gets the sum over the samples."""
     case = (4, 3, 48, FP32, FP32, True, "sample", None, True, False, 1.0)

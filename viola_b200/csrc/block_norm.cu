@@ -128,24 +128,21 @@ namespace {
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Rows of 8-value pieces (16 bytes of a 16-bit type) where every row starts on a 16-byte boundary, single values else.
 // Forward: the work of a row that does not grow with its values (addresses, reductions) is about that of ten values for
 // every thread, so few threads with many values each take the fewest instructions: as many as four pieces a thread, as long
 // as not more lanes idle for it (128 x 256 x 1152, fp32 stream: 120 us with one piece a thread, 85 with three; 4 x 8192 x 4096
 // bf16: 254 and 204).  Backward: a piece takes three times the registers, and warps to hide latency count for more
 // (the same: 145 us with one piece, 237 with three; 375 with one, 530 with four).
-bool norm_shape(int cols, bool wide, bool backward, NormShape& s) {
-  if (cols < 1 || cols > VB_NORM_MAX_COLS || (wide && cols % 8)) return false;
-  const int pieces = wide ? cols / 8 : cols;
-  s.vec = wide ? 8 : 1;
-  if (!wide) {
-    s.v = pieces <= 1024 ? 4 : 16;
-  } else if (backward) {
+bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
+  if (cols < 1 || cols > VB_NORM_MAX_COLS || (!shift && cols % kPiece)) return false;
+  const int pieces = (cols + kPiece - 1) / kPiece;
+  s.shift = shift;
+  if (backward) {
     s.v = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
   } else {
     int best = INT_MAX;
     for (int v = 4; v >= 1; --v) {
-      const int warps = (pieces + 32 * v - 1) / (32 * v), cost = warps * (8 * v + 10);
+      const int warps = (pieces + 32 * v - 1) / (32 * v), cost = warps * (kPiece * v + 10);
       if (warps <= (v == 4 ? 16 : 8) && cost < best) {
         best = cost;
         s.v = v;
@@ -153,15 +150,15 @@ bool norm_shape(int cols, bool wide, bool backward, NormShape& s) {
     }
   }
   s.warps = (pieces + 32 * s.v - 1) / (32 * s.v);
-  s.groups = std::max(1, (backward && wide ? 8 : 4) / s.warps);
-  s.bound = !wide ? (s.v == 4 ? 256 : 1024) : backward || s.warps > 8 ? 512 : 256;
+  s.groups = std::max(1, (backward ? 8 : 4) / s.warps);
+  s.bound = backward || s.warps > 8 ? 512 : 256;
   return true;
 }
 // threads that an SM's registers do for
 int forward_threads(const NormShape& s) {
-  return s.vec == 1 ? 1024 : s.v == 1 ? 768 : s.v == 2 ? 512 : s.v == 3 ? 384 : s.warps > 8 ? 512 : 320;
+  return s.v == 1 ? 768 : s.v == 2 ? 512 : s.v == 3 ? 384 : s.warps > 8 ? 512 : 320;
 }
-int backward_threads(const NormShape& s) { return s.bound == 1024 ? 1024 : 512; }
+constexpr int kBackwardThreads = 512;
 
 // Rows fetched ahead (as many up to three as cost no resident block), shared memory for them and for `areas` fp32 values
 // per column, and blocks that one SM holds where its registers do for `resident_threads`.
@@ -170,12 +167,12 @@ struct NormPlan {
   size_t smem;
 };
 int by_registers(const NormShape& s, int resident_threads) { return std::max(1, resident_threads / s.threads()); }
-NormPlan norm_plan(const NormShape& s, int row_bytes_per_value, int areas, int resident_threads) {
+NormPlan norm_plan(const NormShape& s, int piece_bytes, int areas, int resident_threads) {
   NormPlan p{0, 0, 1, 0};
-  const size_t extra = (size_t)areas * s.v * s.vec * s.threads() * sizeof(float);
+  const size_t extra = (size_t)areas * s.v * kPiece * s.threads() * sizeof(float);
   const int most = by_registers(s, resident_threads);
-  const int slot = s.vec == 8 ? s.v * s.warps * 32 * 8 * row_bytes_per_value : 0;
-  for (p.depth = slot ? 3 : 0;; --p.depth) {
+  const int slot = s.v * s.warps * 32 * piece_bytes;
+  for (p.depth = 3;; --p.depth) {
     p.smem = extra + (p.depth ? (size_t)(p.depth + 1) * s.groups * slot : 0);
     p.resident = std::min(most, (int)(kSharedPerBlock / (p.smem + 2048)));
     if (p.resident == most || p.depth == 0 || (p.depth == 1 && p.resident > 0)) break;
@@ -198,6 +195,7 @@ bool vector_ok(const VbNormVector& v, int cols) {
   return v.data == nullptr || (v.dtype >= kF32 && v.dtype <= kF16 && (v.pitch == 0 || v.pitch >= cols));
 }
 int dtype_size(int dtype) { return dtype == kF32 ? 4 : 2; }
+int piece_bytes(int dtype, bool shift) { return kPiece * dtype_size(dtype) + (shift ? 16 : 0); }      // in a slot
 NormVector to_vector(const VbNormVector& v) {
   return NormVector{v.data, v.dtype, on16(v.data) && v.pitch * dtype_size(v.dtype) % 16 == 0, v.pitch};
 }
@@ -205,11 +203,11 @@ NormVector to_vector(const VbNormVector& v) {
 // Blocks and shared memory of the backward pass: one wave, at least one row to a group
 // Sums of several samples meet in shared memory where row groups share a block or it has the room.
 bool totals_in_shared(const NormShape& s, int rows, int tokens) {
-  return s.groups > 1 || (tokens < rows && 4 * s.v * s.vec * s.threads() * sizeof(float) <= 64 * 1024);
+  return s.groups > 1 || (tokens < rows && 4 * s.v * kPiece * s.threads() * sizeof(float) <= 64 * 1024);
 }
-bool backward_plan(int rows, int cols, int tokens, int x_values, int y_values, bool wide, NormShape& s, NormPlan& p, int& blocks) {
-  if (!norm_shape(cols, wide, true, s)) return false;
-  p = norm_plan(s, x_values + y_values, totals_in_shared(s, rows, tokens) ? 4 : 2, backward_threads(s));
+bool backward_plan(int rows, int cols, int tokens, int bytes, bool shift, NormShape& s, NormPlan& p, int& blocks) {
+  if (!norm_shape(cols, shift, true, s)) return false;
+  p = norm_plan(s, bytes, totals_in_shared(s, rows, tokens) ? 4 : 2, kBackwardThreads);
   blocks = std::min((rows + s.groups - 1) / s.groups, 148 * p.resident);
   return true;
 }
@@ -223,14 +221,10 @@ long long backward_floats(const NormShape& s, int blocks, int rows, int cols, in
 // the most that any types and pointers lead to
 extern "C" long long vb_block_norm_workspace(int rows, int cols, int tokens) {
   if (rows <= 0 || cols <= 0 || tokens <= 0 || rows % tokens || cols > VB_NORM_MAX_COLS) return 0;
-  long long floats = 0;
-  for (const bool wide : {true, false}) {
-    NormShape s;
-    if (!norm_shape(cols, wide, true, s)) continue;
-    const int blocks = std::min((rows + s.groups - 1) / s.groups, 148 * by_registers(s, backward_threads(s)));
-    floats = std::max(floats, backward_floats(s, blocks, rows, cols, tokens));
-  }
-  return floats;
+  NormShape s;
+  if (!norm_shape(cols, true, true, s)) return 0;
+  const int blocks = std::min((rows + s.groups - 1) / s.groups, 148 * by_registers(s, kBackwardThreads));
+  return backward_floats(s, blocks, rows, cols, tokens);
 }
 
 extern "C" int vb_block_norm(const VbBlockNorm* n, cudaStream_t stream) {
@@ -240,10 +234,10 @@ extern "C" int vb_block_norm(const VbBlockNorm* n, cudaStream_t stream) {
       !vector_ok(n->next_scale, n->cols))
     return (int)cudaErrorInvalidValue;
   NormShape s;
-  const bool wide = n->cols % 8 == 0 && on16(n->x) && on16(n->y) && on16(n->out) && on16(n->h);
-  if (!norm_shape(n->cols, wide, false, s)) return (int)cudaErrorInvalidValue;
+  const bool shift = n->cols % kPiece || !on16(n->x) || !on16(n->y) || !on16(n->out) || !on16(n->h);
+  if (!norm_shape(n->cols, shift, false, s)) return (int)cudaErrorInvalidValue;
   if (n->rows == 0) return 0;
-  const NormPlan p = norm_plan(s, dtype_size(n->x_dtype) + (post ? dtype_size(n->y_dtype) : 0), 2, forward_threads(s));
+  const NormPlan p = norm_plan(s, piece_bytes(n->x_dtype, shift) + (post ? piece_bytes(n->y_dtype, shift) : 0), 2, forward_threads(s));
   NormArgs a{};
   a.rows = n->rows; a.cols = n->cols; a.tokens = n->tokens; a.warps = s.warps;
   a.alpha = n->residual_scale; a.eps = n->eps;
@@ -262,14 +256,15 @@ extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGra
       (pre && (n->ru == nullptr || n->x == nullptr)) || (!pre && g->dout == nullptr) || !vector_ok(n->weight, n->cols) ||
       !vector_ok(n->gate, n->cols) || !vector_ok(n->next_weight, n->cols) || !vector_ok(n->next_scale, n->cols))
     return (int)cudaErrorInvalidValue;
-  const bool wide = n->cols % 8 == 0 && on16(n->x) && on16(n->y) && on16(g->dout) && on16(g->dh) && on16(g->dx) && on16(g->dy);
+  const bool shift = n->cols % kPiece || !on16(n->x) || !on16(n->y) || !on16(g->dout) || !on16(g->dh) || !on16(g->dx) || !on16(g->dy);
   if (n->rows == 0) return 0;
   const bool dout = g->dout != nullptr;
   NormShape s;
   NormPlan p;
   int blocks;
-  if (!backward_plan(n->rows, n->cols, n->tokens, dtype_size(n->x_dtype) * ((pre ? 1 : 0) + (dout ? 1 : 0)),
-                     dtype_size(n->y_dtype) * ((post ? 1 : 0) + (pre ? 1 : 0)), wide, s, p, blocks))
+  const int bytes = piece_bytes(n->x_dtype, shift) * ((pre ? 1 : 0) + (dout ? 1 : 0)) +
+                    piece_bytes(n->y_dtype, shift) * ((post ? 1 : 0) + (pre ? 1 : 0));
+  if (!backward_plan(n->rows, n->cols, n->tokens, bytes, shift, s, p, blocks))
     return (int)cudaErrorInvalidValue;
   NormSumArgs t{};
   t.weight[0] = to_vector(n->weight); t.partner[0] = to_vector(n->gate);

@@ -42,50 +42,99 @@ __device__ __forceinline__ void assign(float& to, float v) { to = v; }
 __device__ __forceinline__ void assign(__nv_bfloat16& to, float v) { to = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void assign(__half& to, float v) { to = __float2half_rn(v); }
 
-// VEC neighbouring values as they are stored
-template <typename T, int VEC> struct Piece {
-  static constexpr int kBytes = VEC * (int)sizeof(T);
-  static constexpr bool kWide = kBytes >= 16;
+// A piece: eight neighbouring values of a row as they are stored, one or two 16-byte words.  SHIFT kernels take rows whose
+// pieces do not start on 16-byte boundaries (odd widths, offset views) or whose last piece is cut off: they read and write
+// the aligned words around a piece and shift the bytes into place.
+constexpr int kPiece = 8;
+template <typename T> struct Piece {
+  static constexpr int kWords = kPiece * (int)sizeof(T) / 16;
   union {
-    T value[VEC];
-    uint4 word[kWide ? kBytes / 16 : 1];
+    T value[kPiece];
+    uint4 word[kWords];
+    uint32_t reg[4 * kWords];
   };
   __device__ __forceinline__ Piece() {}
-  __device__ __forceinline__ Piece& operator=(const Piece& other) {
-    if constexpr (kWide) {
-#pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) word[i] = other.word[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) value[i] = other.value[i];
-    }
-    return *this;
-  }
   __device__ __forceinline__ void load(const T* p) {
-    if constexpr (kWide) {
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) word[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) value[i] = p[i];
-    }
+    for (int i = 0; i < kWords; ++i) word[i] = reinterpret_cast<const uint4*>(p)[i];
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (kWide) {
+  __device__ __forceinline__ void load_part(const T* p, int count) {        // single values, zeros behind them
+    clear();
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = word[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) p[i] = value[i];
-    }
+    for (int i = 0; i < kPiece; ++i)
+      if (i < count) value[i] = p[i];
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) assign(value[i], 0.f);
+    for (int i = 0; i < 4 * kWords; ++i) reg[i] = 0u;
   }
   __device__ __forceinline__ float get(int i) const { return as_float(value[i]); }
   __device__ __forceinline__ void set(int i, float v) { assign(value[i], v); }
 };
+
+template <typename T> __device__ __forceinline__ int misalignment(const T* row) { return (int)(reinterpret_cast<uintptr_t>(row) & 15); }
+
+// words[k] becomes the 32-bit word at byte `offset` + 4 k of `words`, for the first N of them; `offset` is even, at most 16,
+// and the same for the whole warp
+template <int N, int M> __device__ __forceinline__ void shift_bytes(uint32_t (&words)[M], int offset) {
+  static_assert(M >= N + 4, "the words behind the last one are shifted in");
+  if (offset & 16) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) words[k] = words[k + 4];
+  }
+  if (offset & 8) {
+#pragma unroll
+    for (int k = 0; k < N + 2; ++k) words[k] = words[k + 2];
+  }
+  if (offset & 4) {
+#pragma unroll
+    for (int k = 0; k < N + 1; ++k) words[k] = words[k + 1];
+  }
+  if (offset & 2) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) words[k] = __funnelshift_r(words[k], words[k + 1], 16);
+  }
+}
+
+// Writes the pieces of a warp's neighbouring columns; every lane takes part, those without columns with `active` false.
+// SHIFT: a lane writes the aligned words that begin in the piece before its own (whose end it gets from the lane below);
+// values of words that are not whole in the warp are written one by one.
+template <typename T, bool SHIFT>
+__device__ __forceinline__ void store_piece(T* row, int c, int cols, bool active, const Piece<T>& piece) {
+  constexpr int kWords = Piece<T>::kWords;
+  if constexpr (!SHIFT) {
+    if (active) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) reinterpret_cast<uint4*>(row + c)[i] = piece.word[i];
+    }
+  } else {
+    const int lane = threadIdx.x & 31, r = misalignment(row), size = (int)sizeof(T);
+    const int begin = c * size - r, end = cols * size;           // of the first word, relative to the row; of the row
+    uint32_t words[4 * kWords + 4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) words[k] = __shfl_up_sync(kAll, piece.reg[4 * (kWords - 1) + k], 1);
+#pragma unroll
+    for (int k = 0; k < 4 * kWords; ++k) words[4 + k] = piece.reg[k];
+    shift_bytes<4 * kWords>(words, 16 - r);
+    bool whole[kWords + 1];
+#pragma unroll
+    for (int g = 0; g <= kWords; ++g) whole[g] = active && begin + 16 * g + 16 <= end;
+    whole[0] = whole[0] && (r == 0 || lane > 0);
+    whole[kWords] = whole[kWords] && lane < 31;                  // the next lane's first word
+    char* at = reinterpret_cast<char*>(row) + begin;
+#pragma unroll
+    for (int g = 0; g < kWords; ++g)
+      if (whole[g]) *reinterpret_cast<uint4*>(at + 16 * g) = make_uint4(words[4 * g], words[4 * g + 1], words[4 * g + 2], words[4 * g + 3]);
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+      const int g = (i * size + r) >> 4;
+      bool covered = whole[0];
+#pragma unroll
+      for (int k = 1; k <= kWords; ++k) covered = g == k ? whole[k] : covered;
+      if (active && c + i < cols && !covered) row[c + i] = piece.value[i];
+    }
+  }
+}
 
 // ---- fetching rows ahead -------------------------------------------------------------------------------------------
 // A thread copies the pieces of the next rows that it will need itself into its own 16-byte places in shared memory
@@ -94,6 +143,10 @@ __device__ __forceinline__ void copy_ahead(uint32_t to, const void* from, bool t
   if (through_l1) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
   else asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// the first `bytes` of a word, zeros behind them
+__device__ __forceinline__ void copy_ahead_part(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait(int pending) {     // all but the youngest `pending` groups have arrived
   if (pending >= 3) asm volatile("cp.async.wait_group 3;" ::: "memory");
@@ -101,29 +154,43 @@ __device__ __forceinline__ void copy_wait(int pending) {     // all but the youn
   else asm volatile("cp.async.wait_group 1;" ::: "memory");
 }
 
-// One tensor's part of a slot: V pieces of VEC values per thread, 16-byte words of neighbouring threads next to each other
-template <typename T, int VEC, int V> struct Strip {
-  static constexpr int kWords = Piece<T, VEC>::kBytes / 16;  // 0: too narrow to be fetched ahead
+// One tensor's part of a slot: V pieces per thread, 16-byte words of neighbouring threads next to each other.  SHIFT: the
+// words around a piece, one more than it has; neighbours fetch the word they share both, the second time from L1.
+template <typename T, int V, bool SHIFT> struct Strip {
+  static constexpr int kWords = Piece<T>::kWords + (SHIFT ? 1 : 0);
   __device__ __forceinline__ static int bytes(int threads) { return V * kWords * threads * 16; }
   // fp32 pieces are two words apart in memory: the halves of a 32-byte sector meet in L1
   __device__ __forceinline__ static void fetch(uint32_t slot, const T* row, int tid, int threads, int cols) {
-    if constexpr (kWords > 0) {
+    const int r = SHIFT ? misalignment(row) : 0;
+    const char* base = reinterpret_cast<const char*>(row) - r;
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = (tid + j * threads) * VEC;
-        if (c < cols)
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * kPiece;
+      if (c < cols) {
 #pragma unroll
-          for (int w = 0; w < kWords; ++w)
-            copy_ahead(slot + ((j * kWords + w) * threads + tid) * 16, row + c + w * (16 / (int)sizeof(T)), kWords > 1);
+        for (int w = 0; w < kWords; ++w) {
+          const uint32_t to = slot + ((j * kWords + w) * threads + tid) * 16;
+          const int from = c * (int)sizeof(T) + 16 * w;
+          if constexpr (SHIFT) {
+            const int left = r + cols * (int)sizeof(T) - from;   // of the row from this word on; nothing behind it is read
+            copy_ahead_part(to, base + (left > 0 ? from : 0), max(0, min(left, 16)));
+          } else {
+            copy_ahead(to, base + from, kWords > 1);
+          }
+        }
       }
     }
   }
-  __device__ __forceinline__ static void take(const unsigned char* slot, int j, int tid, int threads, Piece<T, VEC>& piece) {
-    if constexpr (kWords > 0) {
+  __device__ __forceinline__ static void take(const unsigned char* slot, int j, int tid, int threads, int r, Piece<T>& piece) {
+    uint32_t words[4 * kWords + 4];
 #pragma unroll
-      for (int w = 0; w < kWords; ++w)
-        piece.word[w] = *reinterpret_cast<const uint4*>(slot + ((j * kWords + w) * threads + tid) * 16);
+    for (int w = 0; w < kWords; ++w) {
+      const uint4 v = *reinterpret_cast<const uint4*>(slot + ((j * kWords + w) * threads + tid) * 16);
+      words[4 * w] = v.x; words[4 * w + 1] = v.y; words[4 * w + 2] = v.z; words[4 * w + 3] = v.w;
     }
+    if constexpr (SHIFT) shift_bytes<4 * Piece<T>::kWords>(words, r);
+#pragma unroll
+    for (int k = 0; k < 4 * Piece<T>::kWords; ++k) piece.reg[k] = words[k];
   }
 };
 
@@ -175,85 +242,71 @@ __device__ __forceinline__ void row_sum(float (&v)[N], int warps, int group, flo
 }
 
 // fp32 values of a thread's columns in shared memory, in places of its own (no barrier): value i of piece j
-template <int VEC>
 __device__ __forceinline__ int own_place(int j, int i, int tid, int threads) {
-  return VEC == 1 ? j * threads + tid : ((j * (VEC / 4) + i / 4) * threads + tid) * 4 + i % 4;
+  return ((j * (kPiece / 4) + i / 4) * threads + tid) * 4 + i % 4;
 }
-template <int VEC>
-__device__ __forceinline__ void own_values(const float* area, int j, int tid, int threads, float (&v)[VEC]) {
-  if constexpr (VEC == 1) {
-    v[0] = area[own_place<VEC>(j, 0, tid, threads)];
-  } else {
+__device__ __forceinline__ void own_values(const float* area, int j, int tid, int threads, float (&v)[kPiece]) {
 #pragma unroll
-    for (int w = 0; w < VEC / 4; ++w) {
-      const float4 f = *reinterpret_cast<const float4*>(area + own_place<VEC>(j, 4 * w, tid, threads));
-      v[4 * w] = f.x; v[4 * w + 1] = f.y; v[4 * w + 2] = f.z; v[4 * w + 3] = f.w;
-    }
+  for (int w = 0; w < kPiece / 4; ++w) {
+    const float4 f = *reinterpret_cast<const float4*>(area + own_place(j, 4 * w, tid, threads));
+    v[4 * w] = f.x; v[4 * w + 1] = f.y; v[4 * w + 2] = f.z; v[4 * w + 3] = f.w;
   }
 }
 
 __device__ __forceinline__ float vector_value(const NormVector& v, long long sample, int c, float shift, float otherwise) {
   return v.data != nullptr ? shift + load_as_float(v.data, sample * v.pitch + c, v.dtype) : otherwise;
 }
-// VEC neighbouring values of an optional vector (absent: 1) plus `shift`
-template <int VEC>
-__device__ __forceinline__ void vector_values(const NormVector& v, long long sample, int c, float shift, float (&f)[VEC]) {
+// the values of a piece's columns of an optional vector (absent: 1) plus `shift`; behind the last column 0
+__device__ __forceinline__ void vector_values(const NormVector& v, long long sample, int c, int cols, float shift, float (&f)[kPiece]) {
   if (v.data == nullptr) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+    for (int i = 0; i < kPiece; ++i) f[i] = 1.f;
     return;
   }
   const long long at = sample * v.pitch + c;
-  if (VEC == 8 && v.wide) {
+  if (v.wide && c + kPiece <= cols) {
     if (v.dtype == kF32) {
-      const float4* p = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(v.data) + at);
+      Piece<float> raw;
+      raw.load(reinterpret_cast<const float*>(v.data) + at);
 #pragma unroll
-      for (int w = 0; w < VEC / 4; ++w) {
-        const float4 t = p[w];
-        f[4 * w] = t.x; f[4 * w + 1] = t.y; f[4 * w + 2] = t.z; f[4 * w + 3] = t.w;
-      }
+      for (int i = 0; i < kPiece; ++i) f[i] = raw.get(i) + shift;
     } else {
-      Piece<__nv_bfloat16, VEC> raw;
+      Piece<__nv_bfloat16> raw;
       raw.load(reinterpret_cast<const __nv_bfloat16*>(v.data) + at);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        f[i] = v.dtype == kBF16 ? raw.get(i) : __half2float(__ushort_as_half(__bfloat16_as_ushort(raw.value[i])));
+      for (int i = 0; i < kPiece; ++i)
+        f[i] = (v.dtype == kBF16 ? raw.get(i) : __half2float(__ushort_as_half(__bfloat16_as_ushort(raw.value[i])))) + shift;
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) f[i] = load_as_float(v.data, at + i, v.dtype);
+    for (int i = 0; i < kPiece; ++i) f[i] = c + i < cols ? load_as_float(v.data, at + i, v.dtype) + shift : 0.f;
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) f[i] += shift;
 }
 
 // product of two optional vectors (the second plus `shift`) for the columns of one thread; once per sample
-template <int VEC, int V>
+template <int V>
 __device__ __forceinline__ void store_gain(const NormVector& a, const NormVector& b, float shift, long long sample, int tid,
                                            int threads, int cols, float* area) {
 #pragma unroll 1
   for (int j = 0; j < V; ++j) {
-    const int c = (tid + j * threads) * VEC;
+    const int c = (tid + j * threads) * kPiece;
     if (c < cols) {
-      float f[VEC], g[VEC];
-      vector_values<VEC>(a, sample, c, 0.f, f);
-      vector_values<VEC>(b, sample, c, shift, g);
+      float f[kPiece], g[kPiece];
+      vector_values(a, sample, c, cols, 0.f, f);
+      vector_values(b, sample, c, cols, shift, g);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) area[own_place<VEC>(j, i, tid, threads)] = f[i] * g[i];
+      for (int i = 0; i < kPiece; ++i) area[own_place(j, i, tid, threads)] = f[i] * g[i];
     }
   }
 }
 
-// pieces of rows too wide for registers are walked without unrolling
-#define VB_PIECES _Pragma("unroll (V > 4 ? 1 : V)")
-
-template <typename TX, typename TY, int VEC, int V, int THREADS, bool POST, bool PRE>
+template <typename TX, typename TY, bool SHIFT, int V, int THREADS, bool POST, bool PRE>
 __global__ void __launch_bounds__(THREADS)
 norm_forward_kernel(const NormArgs a) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float buffer[2][1][32];
-  using SX = Strip<TX, VEC, V>;
-  using SY = Strip<TY, VEC, V>;
+  using SX = Strip<TX, V, SHIFT>;
+  using SY = Strip<TY, V, SHIFT>;
   const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
   const int groups = blockDim.x / threads, units = gridDim.x * groups;
   const int per_unit = (a.rows + units - 1) / units;
@@ -273,93 +326,98 @@ norm_forward_kernel(const NormArgs a) {
     copy_commit();
   };
   for (int d = 0; d < a.depth; ++d) fetch(first + d, d);
-  float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * V * VEC * threads;
-  float* next_gains = gains + V * VEC * threads;
+  float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * V * kPiece * threads;
+  float* next_gains = gains + V * kPiece * threads;
   long long sample = first / a.tokens, sample_end = first;
   int turn = 0, head = 0;
   for (long long row = first; row < last; ++row) {
-    Piece<TX, VEC> px[V];
-    Piece<TY, VEC> py[V];
+    Piece<TX> px[V];
+    Piece<TY> py[V];
     const long long base = row * a.cols;
-    if (VEC > 1 && a.depth > 0) {
+    if (a.depth > 0) {
       const int ahead = head + a.depth;
       fetch(row + a.depth, ahead >= slots ? ahead - slots : ahead);
       copy_wait(a.depth);
       const unsigned char* slot = mine + head * a.slot_bytes;
       head = head + 1 == slots ? 0 : head + 1;
-VB_PIECES
+#pragma unroll
       for (int j = 0; j < V; ++j) {
-        SX::take(slot, j, tid, threads, px[j]);
-        if (POST) SY::take(slot + x_bytes, j, tid, threads, py[j]);
+        SX::take(slot, j, tid, threads, misalignment(x + base), px[j]);
+        if (POST) SY::take(slot + x_bytes, j, tid, threads, misalignment(y + base), py[j]);
       }
     } else {
-VB_PIECES
+#pragma unroll
       for (int j = 0; j < V; ++j) {
-        const int c = (tid + j * threads) * VEC;
+        const int c = (tid + j * threads) * kPiece;
         if (c < a.cols) {
-          px[j].load(x + base + c);
-          if (POST) py[j].load(y + base + c);
+          if constexpr (SHIFT) {
+            px[j].load_part(x + base + c, a.cols - c);
+            if (POST) py[j].load_part(y + base + c, a.cols - c);
+          } else {
+            px[j].load(x + base + c);
+            if (POST) py[j].load(y + base + c);
+          }
         }
       }
     }
     if (row >= sample_end) {
       if (row > first) ++sample;
       sample_end = (sample + 1) * a.tokens;
-      if (POST) store_gain<VEC, V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
-      if (PRE) store_gain<VEC, V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
+      if (POST) store_gain<V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
+      if (PRE) store_gain<V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
     }
-    float u[V][VEC], sum[1] = {0.f};
+    float u[V][kPiece], sum[1] = {0.f};
     if (POST) {
-VB_PIECES
-      for (int j = 0; j < V; ++j)
-        if ((tid + j * threads) * VEC < a.cols)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) sum[0] = fmaf(py[j].get(i), py[j].get(i), sum[0]);
+      for (int j = 0; j < V; ++j)
+        if ((tid + j * threads) * kPiece < a.cols)
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i) sum[0] = fmaf(py[j].get(i), py[j].get(i), sum[0]);
       row_sum<1>(sum, a.warps, group, buffer, turn);
       const float ry = rsqrtf(fmaf(sum[0], inverse, a.eps));
       if (tid == 0 && a.ry != nullptr) a.ry[row] = ry;
-VB_PIECES
-      for (int j = 0; j < V; ++j) {
-        const int c = (tid + j * threads) * VEC;
-        if (c < a.cols) {
-          Piece<TX, VEC> o;
-          float gain[VEC];
-          own_values<VEC>(gains, j, tid, threads, gain);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * kPiece;
+        Piece<TX> o;
+        if (c < a.cols) {
+          float gain[kPiece];
+          own_values(gains, j, tid, threads, gain);
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i) {
             u[j][i] = fmaf(a.alpha, px[j].get(i), py[j].get(i) * ry * gain[i]);
             o.set(i, u[j][i]);
           }
-          o.store(reinterpret_cast<TX*>(a.out) + base + c);
         }
+        store_piece<TX, SHIFT>(reinterpret_cast<TX*>(a.out) + base, c, a.cols, c < a.cols, o);
       }
     } else {
-VB_PIECES
+#pragma unroll
       for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) u[j][i] = px[j].get(i);
+        for (int i = 0; i < kPiece; ++i) u[j][i] = px[j].get(i);
     }
     if (PRE) {
       sum[0] = 0.f;
-VB_PIECES
-      for (int j = 0; j < V; ++j)
-        if ((tid + j * threads) * VEC < a.cols)
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) sum[0] = fmaf(u[j][i], u[j][i], sum[0]);
+      for (int j = 0; j < V; ++j)
+        if ((tid + j * threads) * kPiece < a.cols)
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i) sum[0] = fmaf(u[j][i], u[j][i], sum[0]);
       row_sum<1>(sum, a.warps, group, buffer, turn);
       const float ru = rsqrtf(fmaf(sum[0], inverse, a.eps));
       if (tid == 0 && a.ru != nullptr) a.ru[row] = ru;
-VB_PIECES
-      for (int j = 0; j < V; ++j) {
-        const int c = (tid + j * threads) * VEC;
-        if (c < a.cols) {
-          Piece<TY, VEC> o;
-          float gain[VEC];
-          own_values<VEC>(next_gains, j, tid, threads, gain);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o.set(i, u[j][i] * ru * gain[i]);
-          o.store(reinterpret_cast<TY*>(a.h) + base + c);
+      for (int j = 0; j < V; ++j) {
+        const int c = (tid + j * threads) * kPiece;
+        Piece<TY> o;
+        if (c < a.cols) {
+          float gain[kPiece];
+          own_values(next_gains, j, tid, threads, gain);
+#pragma unroll
+          for (int i = 0; i < kPiece; ++i) o.set(i, u[j][i] * ru * gain[i]);
         }
+        store_piece<TY, SHIFT>(reinterpret_cast<TY*>(a.h) + base, c, a.cols, c < a.cols, o);
       }
     }
   }
@@ -375,13 +433,13 @@ VB_PIECES
 // the gradients of the per-sample vectors if it had the whole sample, else parks the sums (place 0: the sample began in
 // an earlier group, 1: it goes on in a later one), and adds them, weighted with the per-sample partner, to the sums of
 // the shared vectors.
-template <typename TX, typename TY, int VEC, int V, int THREADS, bool POST, bool PRE>
+template <typename TX, typename TY, bool SHIFT, int V, int THREADS, bool POST, bool PRE>
 __global__ void __launch_bounds__(THREADS)
 norm_backward_kernel(const NormArgs a) {
   extern __shared__ __align__(16) unsigned char ring[];
   __shared__ float buffer[2][3][32];
-  using SX = Strip<TX, VEC, V>;
-  using SY = Strip<TY, VEC, V>;
+  using SX = Strip<TX, V, SHIFT>;
+  using SY = Strip<TY, V, SHIFT>;
   const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
   const int groups = blockDim.x / threads;
   const TX* x = reinterpret_cast<const TX*>(a.x);
@@ -410,59 +468,62 @@ norm_backward_kernel(const NormArgs a) {
   };
   for (int d = 0; d < a.depth; ++d) fetch(first + d, d);
 
-  float post_sum[V][VEC], pre_sum[V][VEC];
-VB_PIECES
+  float post_sum[V][kPiece], pre_sum[V][kPiece];
+#pragma unroll
   for (int j = 0; j < V; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) post_sum[j][i] = pre_sum[j][i] = 0.f;
+    for (int i = 0; i < kPiece; ++i) post_sum[j][i] = pre_sum[j][i] = 0.f;
   // per group: gains, next gains; then, where sums of several samples or groups meet, sums of S and R
-  const int area = V * VEC * threads;
+  const int area = V * kPiece * threads;
   float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * area;
   float* next_gains = gains + area;
   float* total = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)(groups + group) * 2 * area;
   if (samples && a.totals_shared) {
 #pragma unroll 1
-    for (int k = 0; k < 2 * V * VEC; ++k) total[k * threads + tid] = 0.f;
+    for (int k = 0; k < 2 * V * kPiece; ++k) total[k * threads + tid] = 0.f;
   }
   const long long first_sample = samples ? first / a.tokens : 0;
   auto finish_norm = [&](int n, long long sample, const NormVector& weight, const NormVector& partner, float shift, void* grad,
-                         float (&sum)[V][VEC]) {
+                         float (&sum)[V][kPiece]) {
     const bool fresh = sample == first_sample, before = sample * a.tokens < first, after = (sample + 1) * a.tokens > last;
     float* park = a.parked + ((unit * 2 + (before ? 0 : 1)) * 2 + n) * a.cols;
-VB_PIECES
+#pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (tid + j * threads) * VEC;
+      const int c = (tid + j * threads) * kPiece;
       if (c < a.cols) {
-        float f[VEC];
+        float f[kPiece];
         if (grad != nullptr) {
           if (before || after) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) park[c + i] = sum[j][i];
+            for (int i = 0; i < kPiece; ++i)
+              if (!SHIFT || c + i < a.cols) park[c + i] = sum[j][i];
           } else {
-            vector_values<VEC>(weight, 0, c, 0.f, f);
+            vector_values(weight, 0, c, a.cols, 0.f, f);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) store_from_float(grad, sample * a.cols + c + i, partner.dtype, sum[j][i] * f[i]);
+            for (int i = 0; i < kPiece; ++i)
+              if (!SHIFT || c + i < a.cols) store_from_float(grad, sample * a.cols + c + i, partner.dtype, sum[j][i] * f[i]);
           }
         }
         if (a.sums != nullptr) {
           if (partner.pitch != 0) {
-            vector_values<VEC>(partner, sample, c, shift, f);
+            vector_values(partner, sample, c, a.cols, shift, f);
           } else {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) f[i] = 1.f;
+            for (int i = 0; i < kPiece; ++i) f[i] = 1.f;
           }
           if (a.totals_shared) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) total[n * area + own_place<VEC>(j, i, tid, threads)] += sum[j][i] * f[i];
+            for (int i = 0; i < kPiece; ++i) total[n * area + own_place(j, i, tid, threads)] += sum[j][i] * f[i];
           } else {
             float* to = a.sums + ((long long)blockIdx.x * 2 + n) * a.cols + c;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) to[i] = (fresh ? 0.f : to[i]) + sum[j][i] * f[i];
+            for (int i = 0; i < kPiece; ++i)
+              if (!SHIFT || c + i < a.cols) to[i] = (fresh ? 0.f : to[i]) + sum[j][i] * f[i];
           }
         }
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) sum[j][i] = 0.f;
+      for (int i = 0; i < kPiece; ++i) sum[j][i] = 0.f;
     }
   };
   auto finish_sample = [&](long long sample) {
@@ -470,79 +531,45 @@ VB_PIECES
     if (PRE) finish_norm(1, sample, a.next_weight, a.next_scale, 1.f, a.dnext_scale, pre_sum);
   };
 
-  // single values: the next row's are loaded before this row's are worked on
-  constexpr bool kAhead = VEC == 1 && V <= 4;
-  Piece<TX, VEC> next_x[kAhead ? V : 1], next_d[kAhead ? V : 1];
-  Piece<TY, VEC> next_y[kAhead ? V : 1], next_h[kAhead ? V : 1];
-  auto load_next = [&](long long row) {
-    if constexpr (kAhead) {
-      if (row >= last) return;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const int c = tid + j * threads;
-        const long long at = row * a.cols + c;
-        if (a.dout == nullptr) next_d[j].clear();
-        if (c < a.cols) {
-          if (PRE) next_x[j].load(x + at);
-          if (POST) next_y[j].load(y + at);
-          if (a.dout != nullptr) next_d[j].load(dout + at);
-          if (PRE) next_h[j].load(dh + at);
-        }
-      }
-    }
-  };
-  load_next(first);
   long long sample = first_sample, sample_end = first;
   int turn = 0;
   for (long long row = first; row < last; ++row) {
     const long long base = row * a.cols;
-    Piece<TX, VEC> now_x[kAhead ? V : 1], now_d[kAhead ? V : 1];
-    Piece<TY, VEC> now_y[kAhead ? V : 1], now_h[kAhead ? V : 1];
-    if constexpr (kAhead) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        now_x[j] = next_x[j];
-        now_d[j] = next_d[j];
-        now_y[j] = next_y[j];
-        now_h[j] = next_h[j];
-      }
-      load_next(row + 1);
-    }
     const float ry = POST ? a.ry[row] : 0.f, ru = PRE ? a.ru[row] : 0.f;
     if (row >= sample_end) {
       if (samples && row > first) finish_sample(sample++);
       sample_end = samples ? (sample + 1) * a.tokens : last;
-      if (POST) store_gain<VEC, V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
-      if (PRE) store_gain<VEC, V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
+      if (POST) store_gain<V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
+      if (PRE) store_gain<V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
     }
     const unsigned char* slot = mine + head * a.slot_bytes;
-    if (VEC > 1 && a.depth > 0) {
+    if (a.depth > 0) {
       const int ahead = head + a.depth;
       fetch(row + a.depth, ahead >= slots ? ahead - slots : ahead);
       copy_wait(a.depth);
       head = head + 1 == slots ? 0 : head + 1;
     }
-    float d[V][VEC], yh[V][VEC], uh[V][VEC], sum[3] = {0.f, 0.f, 0.f};
-VB_PIECES
+    float d[V][kPiece], yh[V][kPiece], uh[V][kPiece], sum[3] = {0.f, 0.f, 0.f};
+#pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (tid + j * threads) * VEC;
-      Piece<TX, VEC> px, pd;
-      Piece<TY, VEC> py, ph;
-      float gain[VEC], next_gain[VEC];
+      const int c = (tid + j * threads) * kPiece;
+      Piece<TX> px, pd;
+      Piece<TY> py, ph;
+      float gain[kPiece], next_gain[kPiece];
       if (c < a.cols) {
-        if (POST) own_values<VEC>(gains, j, tid, threads, gain);
-        if (PRE) own_values<VEC>(next_gains, j, tid, threads, next_gain);
+        if (POST) own_values(gains, j, tid, threads, gain);
+        if (PRE) own_values(next_gains, j, tid, threads, next_gain);
         if (a.dout == nullptr) pd.clear();
-        if constexpr (kAhead) {
-          px = now_x[j];
-          pd = now_d[j];
-          py = now_y[j];
-          ph = now_h[j];
-        } else if (VEC > 1 && a.depth > 0) {
-          if (PRE) SX::take(slot, j, tid, threads, px);
-          if (a.dout != nullptr) SX::take(slot + at_dout, j, tid, threads, pd);
-          if (POST) SY::take(slot + at_y, j, tid, threads, py);
-          if (PRE) SY::take(slot + at_dh, j, tid, threads, ph);
+        if (a.depth > 0) {
+          if (PRE) SX::take(slot, j, tid, threads, misalignment(x + base), px);
+          if (a.dout != nullptr) SX::take(slot + at_dout, j, tid, threads, misalignment(dout + base), pd);
+          if (POST) SY::take(slot + at_y, j, tid, threads, misalignment(y + base), py);
+          if (PRE) SY::take(slot + at_dh, j, tid, threads, misalignment(dh + base), ph);
+        } else if constexpr (SHIFT) {
+          if (PRE) px.load_part(x + base + c, a.cols - c);
+          if (POST) py.load_part(y + base + c, a.cols - c);
+          if (a.dout != nullptr) pd.load_part(dout + base + c, a.cols - c);
+          if (PRE) ph.load_part(dh + base + c, a.cols - c);
         } else {
           if (PRE) px.load(x + base + c);
           if (POST) py.load(y + base + c);
@@ -550,7 +577,7 @@ VB_PIECES
           if (PRE) ph.load(dh + base + c);
         }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
+        for (int i = 0; i < kPiece; ++i) {
           float q = 0.f, u;
           d[j][i] = pd.get(i);
           if (POST) {
@@ -573,16 +600,16 @@ VB_PIECES
     row_sum<3>(sum, a.warps, group, buffer, turn);
     const float pull = ru * sum[0] * inverse;                       // ru c
     const float m = POST ? (PRE ? fmaf(-pull, sum[2], sum[1]) : sum[1]) * inverse : 0.f;
-VB_PIECES
-    for (int j = 0; j < V; ++j) {
-      const int c = (tid + j * threads) * VEC;
-      if (c < a.cols) {
-        Piece<TX, VEC> ox;
-        Piece<TY, VEC> oy;
-        float gain[VEC];
-        if (POST) own_values<VEC>(gains, j, tid, threads, gain);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
+    for (int j = 0; j < V; ++j) {
+      const int c = (tid + j * threads) * kPiece;
+      Piece<TX> ox;
+      Piece<TY> oy;
+      if (c < a.cols) {
+        float gain[kPiece];
+        if (POST) own_values(gains, j, tid, threads, gain);
+#pragma unroll
+        for (int i = 0; i < kPiece; ++i) {
           const float whole = PRE ? fmaf(-pull, uh[j][i], d[j][i]) : d[j][i];
           ox.set(i, POST ? a.alpha * whole : whole);
           if (POST) {
@@ -590,21 +617,22 @@ VB_PIECES
             post_sum[j][i] = fmaf(whole, yh[j][i], post_sum[j][i]);
           }
         }
-        if (a.dx != nullptr) ox.store(reinterpret_cast<TX*>(a.dx) + base + c);
-        if (POST && a.dy != nullptr) oy.store(reinterpret_cast<TY*>(a.dy) + base + c);
       }
+      if (a.dx != nullptr) store_piece<TX, SHIFT>(reinterpret_cast<TX*>(a.dx) + base, c, a.cols, c < a.cols, ox);
+      if (POST && a.dy != nullptr) store_piece<TY, SHIFT>(reinterpret_cast<TY*>(a.dy) + base, c, a.cols, c < a.cols, oy);
     }
   }
   if (samples && first < last) finish_sample(sample);
   if (a.sums == nullptr || (samples && !a.totals_shared)) return;
   float* to = a.sums + (long long)blockIdx.x * 2 * a.cols;
   if (!samples && groups == 1) {
-VB_PIECES
+#pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (tid + j * threads) * VEC;
+      const int c = (tid + j * threads) * kPiece;
       if (c < a.cols)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
+        for (int i = 0; i < kPiece; ++i) {
+          if (SHIFT && c + i >= a.cols) continue;
           to[c + i] = POST ? post_sum[j][i] : 0.f;
           to[a.cols + c + i] = PRE ? pre_sum[j][i] : 0.f;
         }
@@ -612,22 +640,22 @@ VB_PIECES
     return;
   }
   if (!samples) {
-VB_PIECES
+#pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        total[own_place<VEC>(j, i, tid, threads)] = POST ? post_sum[j][i] : 0.f;
-        total[area + own_place<VEC>(j, i, tid, threads)] = PRE ? pre_sum[j][i] : 0.f;
+      for (int i = 0; i < kPiece; ++i) {
+        total[own_place(j, i, tid, threads)] = POST ? post_sum[j][i] : 0.f;
+        total[area + own_place(j, i, tid, threads)] = PRE ? pre_sum[j][i] : 0.f;
       }
   }
   __syncthreads();
   // the first group adds the groups' sums in order
   if (group == 0) {
 #pragma unroll 1
-    for (int k = 0; k < 2 * V * VEC; ++k) {
-      const int n = k / (V * VEC), j = k / VEC % V, i = k % VEC, c = (tid + j * threads) * VEC + i;
+    for (int k = 0; k < 2 * V * kPiece; ++k) {
+      const int n = k / (V * kPiece), j = k / kPiece % V, i = k % kPiece, c = (tid + j * threads) * kPiece + i;
       if (c < a.cols) {
-        const float* from = total + n * area + own_place<VEC>(j, i, tid, threads);
+        const float* from = total + n * area + own_place(j, i, tid, threads);
         float s = from[0];
         for (int g = 1; g < groups; ++g) s += from[(size_t)g * 2 * area];
         to[n * a.cols + c] = s;
@@ -639,7 +667,8 @@ VB_PIECES
 constexpr int kSharedPerBlock = 227 * 1024;
 
 struct NormShape {
-  int vec, v, warps, groups;   // values per access, accesses per thread, warps per row, rows a block works on at a time
+  bool shift;                  // pieces do not all start on 16-byte boundaries, or the last is cut off
+  int v, warps, groups;        // pieces per thread, warps per row, rows a block works on at a time
   int bound;                   // threads that the kernel's template is built for
   int threads() const { return warps * groups * 32; }
 };
@@ -670,35 +699,38 @@ void launch_kernel(const NormArgs& a, const NormLaunch& l) {
   Kernel<<<l.blocks, l.threads, l.smem, l.stream>>>(a);
 }
 
-template <bool BACKWARD, typename TX, typename TY, int VEC, int V, int THREADS>
+template <bool BACKWARD, typename TX, typename TY, bool SHIFT, int V, int THREADS>
 void launch_norms(const NormArgs& a, const NormLaunch& l) {
   if constexpr (BACKWARD) {
-    if (l.post && l.pre) launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, true, true>>(a, l);
-    else if (l.post) launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, true, false>>(a, l);
-    else launch_kernel<norm_backward_kernel<TX, TY, VEC, V, THREADS, false, true>>(a, l);
+    if (l.post && l.pre) launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
+    else if (l.post) launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
+    else launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
   } else {
-    if (l.post && l.pre) launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, true, true>>(a, l);
-    else if (l.post) launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, true, false>>(a, l);
-    else launch_kernel<norm_forward_kernel<TX, TY, VEC, V, THREADS, false, true>>(a, l);
+    if (l.post && l.pre) launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
+    else if (l.post) launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
+    else launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
+  }
+}
+
+template <typename TX, typename TY, bool SHIFT>
+void launch_aligned(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
+  if (l.backward) {
+    if (s.v == 1) launch_norms<true, TX, TY, SHIFT, 1, 512>(a, l);
+    else if (s.v == 2) launch_norms<true, TX, TY, SHIFT, 2, 512>(a, l);
+    else launch_norms<true, TX, TY, SHIFT, 4, 512>(a, l);
+  } else {
+    if (s.v == 1) launch_norms<false, TX, TY, SHIFT, 1, 256>(a, l);
+    else if (s.v == 2) launch_norms<false, TX, TY, SHIFT, 2, 256>(a, l);
+    else if (s.v == 3) launch_norms<false, TX, TY, SHIFT, 3, 256>(a, l);
+    else if (s.bound == 256) launch_norms<false, TX, TY, SHIFT, 4, 256>(a, l);
+    else launch_norms<false, TX, TY, SHIFT, 4, 512>(a, l);
   }
 }
 
 template <typename TX, typename TY>
 void launch_shape(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
-  if (s.vec == 1) {
-    if (l.backward) s.v == 4 ? launch_norms<true, TX, TY, 1, 4, 256>(a, l) : launch_norms<true, TX, TY, 1, 16, 1024>(a, l);
-    else s.v == 4 ? launch_norms<false, TX, TY, 1, 4, 256>(a, l) : launch_norms<false, TX, TY, 1, 16, 1024>(a, l);
-  } else if (l.backward) {
-    if (s.v == 1) launch_norms<true, TX, TY, 8, 1, 512>(a, l);
-    else if (s.v == 2) launch_norms<true, TX, TY, 8, 2, 512>(a, l);
-    else launch_norms<true, TX, TY, 8, 4, 512>(a, l);
-  } else {
-    if (s.v == 1) launch_norms<false, TX, TY, 8, 1, 256>(a, l);
-    else if (s.v == 2) launch_norms<false, TX, TY, 8, 2, 256>(a, l);
-    else if (s.v == 3) launch_norms<false, TX, TY, 8, 3, 256>(a, l);
-    else if (s.bound == 256) launch_norms<false, TX, TY, 8, 4, 256>(a, l);
-    else launch_norms<false, TX, TY, 8, 4, 512>(a, l);
-  }
+  if (s.shift) launch_aligned<TX, TY, true>(a, s, l);
+  else launch_aligned<TX, TY, false>(a, s, l);
 }
 
 }  // namespace vb
