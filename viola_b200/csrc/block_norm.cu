@@ -13,11 +13,11 @@
 
 namespace vb {
 
-extern template void launch_shape<float, float>(const NormArgs&, const NormShape&, const NormLaunch&);
-extern template void launch_shape<float, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
-extern template void launch_shape<float, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
-extern template void launch_shape<__nv_bfloat16, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
-extern template void launch_shape<__half, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
+extern template int launch_shape<float, float>(const NormArgs&, const NormShape&, const NormLaunch&);
+extern template int launch_shape<float, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
+extern template int launch_shape<float, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
+extern template int launch_shape<__nv_bfloat16, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
+extern template int launch_shape<__half, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
 
 struct NormSumArgs {
   int rows, cols, tokens;
@@ -181,14 +181,14 @@ NormPlan norm_plan(const NormShape& s, int piece_bytes, int areas, int resident_
   return p;
 }
 
+// returns the number of blocks launched, 0 for types that do not go together
 int launch_types(const NormArgs& a, int x_dtype, int y_dtype, const NormShape& s, const NormLaunch& l) {
-  if (x_dtype == kF32 && y_dtype == kF32) launch_shape<float, float>(a, s, l);
-  else if (x_dtype == kF32 && y_dtype == kBF16) launch_shape<float, __nv_bfloat16>(a, s, l);
-  else if (x_dtype == kF32 && y_dtype == kF16) launch_shape<float, __half>(a, s, l);
-  else if (x_dtype == kBF16 && y_dtype == kBF16) launch_shape<__nv_bfloat16, __nv_bfloat16>(a, s, l);
-  else if (x_dtype == kF16 && y_dtype == kF16) launch_shape<__half, __half>(a, s, l);
-  else return (int)cudaErrorInvalidValue;
-  return (int)cudaGetLastError();
+  if (x_dtype == kF32 && y_dtype == kF32) return launch_shape<float, float>(a, s, l);
+  if (x_dtype == kF32 && y_dtype == kBF16) return launch_shape<float, __nv_bfloat16>(a, s, l);
+  if (x_dtype == kF32 && y_dtype == kF16) return launch_shape<float, __half>(a, s, l);
+  if (x_dtype == kBF16 && y_dtype == kBF16) return launch_shape<__nv_bfloat16, __nv_bfloat16>(a, s, l);
+  if (x_dtype == kF16 && y_dtype == kF16) return launch_shape<__half, __half>(a, s, l);
+  return 0;
 }
 
 bool vector_ok(const VbNormVector& v, int cols) {
@@ -200,7 +200,7 @@ NormVector to_vector(const VbNormVector& v) {
   return NormVector{v.data, v.dtype, on16(v.data) && v.pitch * dtype_size(v.dtype) % 16 == 0, v.pitch};
 }
 
-// Blocks and shared memory of the backward pass: one wave, at least one row to a group
+// Shared memory of the backward pass and the most blocks: one wave, at least one row to a group
 // Sums of several samples meet in shared memory where row groups share a block or it has the room.
 bool totals_in_shared(const NormShape& s, int rows, int tokens) {
   return s.groups > 1 || (tokens < rows && 4 * s.v * kPiece * s.threads() * sizeof(float) <= 64 * 1024);
@@ -246,8 +246,10 @@ extern "C" int vb_block_norm(const VbBlockNorm* n, cudaStream_t stream) {
   a.next_weight = to_vector(n->next_weight); a.next_scale = to_vector(n->next_scale);
   a.out = n->out; a.h = n->h; a.ry = n->ry; a.ru = n->ru;
   a.depth = p.depth; a.slot_bytes = p.slot_bytes;
-  const int blocks = std::min((n->rows + s.groups - 1) / s.groups, 148 * p.resident);
-  return launch_types(a, n->x_dtype, n->y_dtype, s, NormLaunch{false, post, pre, blocks, s.threads(), p.smem, stream});
+  const int blocks = (n->rows + s.groups - 1) / s.groups;
+  if (launch_types(a, n->x_dtype, n->y_dtype, s, NormLaunch{false, post, pre, blocks, s.threads(), p.smem, stream}) == 0)
+    return (int)cudaErrorInvalidValue;
+  return (int)cudaGetLastError();
 }
 
 extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGrads* g, cudaStream_t stream) {
@@ -294,8 +296,9 @@ extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGra
   if (t.partner[1].pitch != 0) a.dnext_scale = t.dpartner[1];
   a.totals_shared = totals_in_shared(s, n->rows, n->tokens);
   a.depth = p.depth; a.slot_bytes = p.slot_bytes;
-  const int rc = launch_types(a, n->x_dtype, n->y_dtype, s,
-                              NormLaunch{true, post, pre, blocks, s.threads(), p.smem, stream});
+  blocks = launch_types(a, n->x_dtype, n->y_dtype, s, NormLaunch{true, post, pre, blocks, s.threads(), p.smem, stream});
+  if (blocks == 0) return (int)cudaErrorInvalidValue;
+  const int rc = (int)cudaGetLastError();
   if (rc != 0 || !(shared || per_sample)) return rc;
   t.rows = n->rows; t.cols = n->cols; t.tokens = n->tokens;
   t.blocks = shared ? blocks : 0;

@@ -688,49 +688,65 @@ void allow_shared() {
 
 struct NormLaunch {
   bool backward, post, pre;
-  int blocks, threads;
+  int blocks, threads;         // blocks: as many as there is room for, at most these
   size_t smem;
   cudaStream_t stream;
 };
 
+// blocks of a kernel that one SM holds at once; the answer for the last shape is kept
 template <auto Kernel>
-void launch_kernel(const NormArgs& a, const NormLaunch& l) {
+int resident_blocks(int threads, size_t smem) {
+  static std::atomic<unsigned long long> last{0};      // threads (16 bits), smem (32), blocks (16)
+  const unsigned long long key = (unsigned long long)threads << 48 | (unsigned long long)smem << 16;
+  const unsigned long long seen = last.load(std::memory_order_relaxed);
+  if ((seen & ~0xffffull) == key) return (int)(seen & 0xffffull);
+  int blocks = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, Kernel, threads, smem) != cudaSuccess) return 1;
+  blocks = blocks > 1 ? blocks : 1;
+  last.store(key | (unsigned long long)blocks, std::memory_order_relaxed);
+  return blocks;
+}
+
+// one wave; returns the number of blocks
+template <auto Kernel>
+int launch_kernel(const NormArgs& a, const NormLaunch& l) {
   if (l.smem > 48 * 1024 - 1024) allow_shared<Kernel>();
-  Kernel<<<l.blocks, l.threads, l.smem, l.stream>>>(a);
+  const int room = 148 * resident_blocks<Kernel>(l.threads, l.smem), blocks = l.blocks < room ? l.blocks : room;
+  Kernel<<<blocks, l.threads, l.smem, l.stream>>>(a);
+  return blocks;
 }
 
 template <bool BACKWARD, typename TX, typename TY, bool SHIFT, int V, int THREADS>
-void launch_norms(const NormArgs& a, const NormLaunch& l) {
+int launch_norms(const NormArgs& a, const NormLaunch& l) {
   if constexpr (BACKWARD) {
-    if (l.post && l.pre) launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
-    else if (l.post) launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
-    else launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
+    if (l.post && l.pre) return launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
+    if (l.post) return launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
+    return launch_kernel<norm_backward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
   } else {
-    if (l.post && l.pre) launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
-    else if (l.post) launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
-    else launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
+    if (l.post && l.pre) return launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, true>>(a, l);
+    if (l.post) return launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, true, false>>(a, l);
+    return launch_kernel<norm_forward_kernel<TX, TY, SHIFT, V, THREADS, false, true>>(a, l);
   }
 }
 
 template <typename TX, typename TY, bool SHIFT>
-void launch_aligned(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
+int launch_aligned(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
   if (l.backward) {
-    if (s.v == 1) launch_norms<true, TX, TY, SHIFT, 1, 512>(a, l);
-    else if (s.v == 2) launch_norms<true, TX, TY, SHIFT, 2, 512>(a, l);
-    else launch_norms<true, TX, TY, SHIFT, 4, 512>(a, l);
+    if (s.v == 1) return launch_norms<true, TX, TY, SHIFT, 1, 512>(a, l);
+    if (s.v == 2) return launch_norms<true, TX, TY, SHIFT, 2, 512>(a, l);
+    return launch_norms<true, TX, TY, SHIFT, 4, 512>(a, l);
   } else {
-    if (s.v == 1) launch_norms<false, TX, TY, SHIFT, 1, 256>(a, l);
-    else if (s.v == 2) launch_norms<false, TX, TY, SHIFT, 2, 256>(a, l);
-    else if (s.v == 3) launch_norms<false, TX, TY, SHIFT, 3, 256>(a, l);
-    else if (s.bound == 256) launch_norms<false, TX, TY, SHIFT, 4, 256>(a, l);
-    else launch_norms<false, TX, TY, SHIFT, 4, 512>(a, l);
+    if (s.v == 1) return launch_norms<false, TX, TY, SHIFT, 1, 256>(a, l);
+    if (s.v == 2) return launch_norms<false, TX, TY, SHIFT, 2, 256>(a, l);
+    if (s.v == 3) return launch_norms<false, TX, TY, SHIFT, 3, 256>(a, l);
+    if (s.bound == 256) return launch_norms<false, TX, TY, SHIFT, 4, 256>(a, l);
+    return launch_norms<false, TX, TY, SHIFT, 4, 512>(a, l);
   }
 }
 
 template <typename TX, typename TY>
-void launch_shape(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
-  if (s.shift) launch_aligned<TX, TY, true>(a, s, l);
-  else launch_aligned<TX, TY, false>(a, s, l);
+int launch_shape(const NormArgs& a, const NormShape& s, const NormLaunch& l) {
+  return s.shift ? launch_aligned<TX, TY, true>(a, s, l) : launch_aligned<TX, TY, false>(a, s, l);
 }
 
 }  // namespace vb

@@ -2,5 +2,5 @@
 #include "block_norm.cuh"
 
 namespace vb {
-template void launch_shape<__nv_bfloat16, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
+template int launch_shape<__nv_bfloat16, __nv_bfloat16>(const NormArgs&, const NormShape&, const NormLaunch&);
 }  // namespace vb

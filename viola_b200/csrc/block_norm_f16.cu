@@ -2,5 +2,5 @@
 #include "block_norm.cuh"
 
 namespace vb {
-template void launch_shape<__half, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
+template int launch_shape<__half, __half>(const NormArgs&, const NormShape&, const NormLaunch&);
 }  // namespace vb

@@ -2,5 +2,5 @@
 #include "block_norm.cuh"
 
 namespace vb {
-template void launch_shape<float, float>(const NormArgs&, const NormShape&, const NormLaunch&);
+template int launch_shape<float, float>(const NormArgs&, const NormShape&, const NormLaunch&);
 }  // namespace vb
