@@ -194,51 +194,73 @@ template <typename T, int V, bool SHIFT> struct Strip {
   }
 };
 
-// Sums N values over the warps of a row; every thread gets them.  `turn` alternates between two buffers, so that one
-// barrier per call is enough: a warp can only reach the buffer's next use through the other buffer's barrier.
-// Rows that a block works on at the same time meet at barriers of their own.
-template <int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], int warps, int group, float (*buffer)[N][32], int& turn) {
-#pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(kAll, v[n], o);
-  if (warps == 1) return;
-  const int lane = threadIdx.x & 31, first = group * warps;
-  if (lane == 0) {
-#pragma unroll
-    for (int n = 0; n < N; ++n) buffer[turn][n][threadIdx.x >> 5] = v[n];
-  }
-  // (named one by one: a barrier number in a register would reserve all sixteen for the block)
+// Sums over the warps of a row; every thread gets them.  `turn` alternates between two buffers, so that one barrier per
+// call is enough: a warp can only reach the buffer's next use through the other buffer's barrier.  Rows that a block works
+// on at the same time meet at barriers of their own (named one by one: a barrier number in a register would reserve all
+// sixteen for the block).
+__device__ __forceinline__ void row_barrier(int warps, int group) {
   if (group == 0) asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
   else if (group == 1) asm volatile("bar.sync 2, %0;" ::"r"(warps * 32) : "memory");
   else if (group == 2) asm volatile("bar.sync 3, %0;" ::"r"(warps * 32) : "memory");
   else asm volatile("bar.sync 4, %0;" ::"r"(warps * 32) : "memory");
+}
+__device__ __forceinline__ float row_sum(float v, int warps, int group, float (*buffer)[32], int& turn) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  if (warps == 1) return v;
+  const int lane = threadIdx.x & 31, first = group * warps;
+  if (lane == 0) buffer[turn][threadIdx.x >> 5] = v;
+  row_barrier(warps, group);
   if (warps <= 4) {
+    v = buffer[turn][first] + buffer[turn][first + 1];
+    if (warps > 2) v += buffer[turn][first + 2];
+    if (warps > 3) v += buffer[turn][first + 3];
+  } else {                                      // at most 16; every warp adds the warps' sums for itself
+    v = (lane & 15) < warps ? buffer[turn][first + (lane & 15)] : 0.f;
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      v[n] = buffer[turn][n][first] + buffer[turn][n][first + 1];
-      if (warps > 2) v[n] += buffer[turn][n][first + 2];
-      if (warps > 3) v[n] += buffer[turn][n][first + 3];
-    }
-  } else {
-    // every warp adds the warps' sums for itself: one value a lane, 8, 16 or 32 lanes
-#pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = lane < warps ? buffer[turn][n][first + lane] : 0.f;
-    if (warps > 16)
-#pragma unroll
-      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], 16);
-    if (warps > 8)
-#pragma unroll
-      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], 8);
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1)
-#pragma unroll
-      for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(kAll, v[n], o);
-#pragma unroll
-    for (int n = 0; n < N; ++n) v[n] = __shfl_sync(kAll, v[n], 0);
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
   }
   turn ^= 1;
+  return v;
+}
+// Three sums at once: the first two exchanges leave every eight lanes with one of them, so that three values cost 6 shuffles
+// and not 15, and the sums of up to 16 warps 10 (8 warps: 6).
+__device__ __forceinline__ void row_sum(float (&v)[3], int warps, int group, float (*buffer)[3][32], int& turn) {
+  const int lane = threadIdx.x & 31, first = group * warps;
+  const bool upper = lane & 16, odd = lane & 8;
+  float x = __shfl_xor_sync(kAll, upper ? v[0] : v[2], 16), y = __shfl_xor_sync(kAll, v[1], 16);
+  x += upper ? v[2] : v[0];                     // lanes 0-15: the first sum, 16-31: the third
+  y = upper ? 0.f : y + v[1];                   // lanes 0-15: the second
+  float keep = (odd ? y : x) + __shfl_xor_sync(kAll, odd ? x : y, 8);
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) keep += __shfl_xor_sync(kAll, keep, o);
+  if (warps > 1) {
+    if (lane < 24 && (lane & 7) == 0) buffer[turn][lane >> 3][threadIdx.x >> 5] = keep;
+    row_barrier(warps, group);
+    if (warps <= 8) {
+      keep = lane < 24 && (lane & 7) < warps ? buffer[turn][lane >> 3][first + (lane & 7)] : 0.f;
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) keep += __shfl_xor_sync(kAll, keep, o);
+    } else {
+      const bool there = (lane & 15) < warps;
+      keep = there ? buffer[turn][lane >> 4][first + (lane & 15)] : 0.f;
+      float third = there ? buffer[turn][2][first + (lane & 15)] : 0.f;
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) {
+        keep += __shfl_xor_sync(kAll, keep, o);
+        third += __shfl_xor_sync(kAll, third, o);
+      }
+      v[0] = __shfl_sync(kAll, keep, 0);
+      v[1] = __shfl_sync(kAll, keep, 16);
+      v[2] = third;
+      turn ^= 1;
+      return;
+    }
+    turn ^= 1;
+  }
+  v[0] = __shfl_sync(kAll, keep, 0);
+  v[1] = __shfl_sync(kAll, keep, 8);
+  v[2] = __shfl_sync(kAll, keep, 16);
 }
 
 // fp32 values of a thread's columns in shared memory, in places of its own (no barrier): value i of piece j
@@ -304,7 +326,7 @@ template <typename TX, typename TY, bool SHIFT, int V, int THREADS, bool POST, b
 __global__ void __launch_bounds__(THREADS)
 norm_forward_kernel(const NormArgs a) {
   extern __shared__ __align__(16) unsigned char ring[];
-  __shared__ float buffer[2][1][32];
+  __shared__ float buffer[2][32];
   using SX = Strip<TX, V, SHIFT>;
   using SY = Strip<TY, V, SHIFT>;
   const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
@@ -366,15 +388,14 @@ norm_forward_kernel(const NormArgs a) {
       if (POST) store_gain<V>(a.weight, a.gate, 0.f, sample, tid, threads, a.cols, gains);
       if (PRE) store_gain<V>(a.next_weight, a.next_scale, 1.f, sample, tid, threads, a.cols, next_gains);
     }
-    float u[V][kPiece], sum[1] = {0.f};
+    float u[V][kPiece], sum = 0.f;
     if (POST) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((tid + j * threads) * kPiece < a.cols)
 #pragma unroll
-          for (int i = 0; i < kPiece; ++i) sum[0] = fmaf(py[j].get(i), py[j].get(i), sum[0]);
-      row_sum<1>(sum, a.warps, group, buffer, turn);
-      const float ry = rsqrtf(fmaf(sum[0], inverse, a.eps));
+          for (int i = 0; i < kPiece; ++i) sum = fmaf(py[j].get(i), py[j].get(i), sum);
+      const float ry = rsqrtf(fmaf(row_sum(sum, a.warps, group, buffer, turn), inverse, a.eps));
       if (tid == 0 && a.ry != nullptr) a.ry[row] = ry;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -398,14 +419,13 @@ norm_forward_kernel(const NormArgs a) {
         for (int i = 0; i < kPiece; ++i) u[j][i] = px[j].get(i);
     }
     if (PRE) {
-      sum[0] = 0.f;
+      sum = 0.f;
 #pragma unroll
       for (int j = 0; j < V; ++j)
         if ((tid + j * threads) * kPiece < a.cols)
 #pragma unroll
-          for (int i = 0; i < kPiece; ++i) sum[0] = fmaf(u[j][i], u[j][i], sum[0]);
-      row_sum<1>(sum, a.warps, group, buffer, turn);
-      const float ru = rsqrtf(fmaf(sum[0], inverse, a.eps));
+          for (int i = 0; i < kPiece; ++i) sum = fmaf(u[j][i], u[j][i], sum);
+      const float ru = rsqrtf(fmaf(row_sum(sum, a.warps, group, buffer, turn), inverse, a.eps));
       if (tid == 0 && a.ru != nullptr) a.ru[row] = ru;
 #pragma unroll
       for (int j = 0; j < V; ++j) {
@@ -597,7 +617,7 @@ norm_backward_kernel(const NormArgs a) {
         }
       }
     }
-    row_sum<3>(sum, a.warps, group, buffer, turn);
+    row_sum(sum, a.warps, group, buffer, turn);
     const float pull = ru * sum[0] * inverse;                       // ru c
     const float m = POST ? (PRE ? fmaf(-pull, sum[2], sum[1]) : sum[1]) * inverse : 0.f;
 #pragma unroll
@@ -617,9 +637,15 @@ norm_backward_kernel(const NormArgs a) {
             post_sum[j][i] = fmaf(whole, yh[j][i], post_sum[j][i]);
           }
         }
+        if constexpr (!SHIFT) {
+          if (a.dx != nullptr) store_piece<TX, SHIFT>(reinterpret_cast<TX*>(a.dx) + base, c, a.cols, true, ox);
+          if (POST && a.dy != nullptr) store_piece<TY, SHIFT>(reinterpret_cast<TY*>(a.dy) + base, c, a.cols, true, oy);
+        }
       }
-      if (a.dx != nullptr) store_piece<TX, SHIFT>(reinterpret_cast<TX*>(a.dx) + base, c, a.cols, c < a.cols, ox);
-      if (POST && a.dy != nullptr) store_piece<TY, SHIFT>(reinterpret_cast<TY*>(a.dy) + base, c, a.cols, c < a.cols, oy);
+      if constexpr (SHIFT) {
+        if (a.dx != nullptr) store_piece<TX, SHIFT>(reinterpret_cast<TX*>(a.dx) + base, c, a.cols, c < a.cols, ox);
+        if (POST && a.dy != nullptr) store_piece<TY, SHIFT>(reinterpret_cast<TY*>(a.dy) + base, c, a.cols, c < a.cols, oy);
+      }
     }
   }
   if (samples && first < last) finish_sample(sample);
