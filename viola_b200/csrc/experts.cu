@@ -940,10 +940,10 @@ extern "C" int vb_expert_plan(const void* indices, int is_long, int n, int exper
   return (int)cudaGetLastError();
 }
 
-// Blocks of 8 warps for so many items of a warp.  32 blocks an SM, four times what is resident, even out the tail:
-// dispatch of 32768 x 2048 bf16 to four experts 113 us at 8 blocks an SM, 107 us (96 % of the copy rate) at 32.
+// Blocks of 8 warps for so many items of a warp.  32 blocks an SM, four times what is resident, even out the tail of long
+// runs: dispatch of 32768 x 2048 bf16 to four experts 113 us at 8 blocks an SM, 107 us (96 % of the copy rate) at 32.
 static int row_blocks(long long items) {
-  const long long most = items >= 148LL * 32 * 8 * 2 ? 148 * 32 : 148 * 8;
+  const long long most = items >= 148LL * 32 * 8 ? 148 * 32 : 148 * 8;
   return (int)std::max<long long>(1, std::min<long long>((items + 7) / 8, most));
 }
 // Packs a lane: a whole row (up to 8 a lane) to a warp where that leaves every SM 16 warps, so that all its loads are in
@@ -1014,22 +1014,22 @@ extern "C" int vb_expert_combine_backward(const void* dout, const void* rows, in
   if (tokens == 0) return 0;
   const int size = dtype == kF32 ? 4 : 2, pack = 16 / size;
   const bool wide = width % pack == 0 && aligned_to(rows, 16) && aligned_to(dout, 16) && (drows == nullptr || aligned_to(drows, 16));
-  const int packs = wide ? width / pack : width, most = row_packs(packs, tokens);
+  // (at most 5 packs a lane: 32768 x 2048 bf16, four choices, 195 us with two warps a token, 204 to 249 with one of 8 packs)
+  const int packs = wide ? width / pack : width, most = std::min(5, row_packs(packs, tokens));
   int team = 1;
   while (team < 8 && packs > team * 32 * most) team *= 2;
-  const int blocks = row_blocks((long long)tokens * team);
+  const int per_lane = (packs + team * 32 - 1) / (team * 32), blocks = row_blocks((long long)tokens * team);
   VB_FLOAT_SWITCH(dtype, {
     constexpr int N = 16 / (int)sizeof(T);
     auto launch = [&](auto kernel) {
       kernel<<<blocks, 256, 0, stream>>>((const T*)dout, (const T*)rows, width, tokens, top_k, team, positions, offsets, experts,
                                          weights, weight_dtype, (T*)drows, dweights);
     };
-    if (wide && most == 2) launch(combine_backward_kernel<T, N, 2>);
-    else if (wide && most == 5) launch(combine_backward_kernel<T, N, 5>);
-    else if (wide) launch(combine_backward_kernel<T, N, 8>);
-    else if (most == 2) launch(combine_backward_kernel<T, 1, 2>);
-    else if (most == 5) launch(combine_backward_kernel<T, 1, 5>);
-    else launch(combine_backward_kernel<T, 1, 8>);
+    if (wide && per_lane <= 2) launch(combine_backward_kernel<T, N, 2>);
+    else if (wide && per_lane <= 4) launch(combine_backward_kernel<T, N, 4>);
+    else if (wide) launch(combine_backward_kernel<T, N, 5>);
+    else if (per_lane <= 2) launch(combine_backward_kernel<T, 1, 2>);
+    else launch(combine_backward_kernel<T, 1, 4>);
   });
   return (int)cudaGetLastError();
 }
