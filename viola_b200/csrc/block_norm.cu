@@ -130,9 +130,9 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Forward: the work of a row that does not grow with its values (addresses, reductions) is about that of ten values for
 // every thread, so few threads with many values each take the fewest instructions: as many as four pieces a thread, as long
-// as not more lanes idle for it (128 x 256 x 1152, fp32 stream: 120 us with one piece a thread, 85 with three; 4 x 8192 x 4096
-// bf16: 254 and 204).  Backward: a piece takes three times the registers, and warps to hide latency count for more
-// (the same: 145 us with one piece, 237 with three; 375 with one, 530 with four).
+// as not more lanes idle for it (128 x 256 x 1152, fp32 stream: 120 us with one piece a thread, 86 with three; 4 x 8192 x 4096
+// bf16: 254 and 202).  Backward: a piece takes three times the registers, and warps to hide latency count for more
+// (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four).
 bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
   if (cols < 1 || cols > VB_NORM_MAX_COLS || (!shift && cols % kPiece)) return false;
   const int pieces = (cols + kPiece - 1) / kPiece;

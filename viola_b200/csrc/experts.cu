@@ -168,8 +168,9 @@ template <int V> __device__ __forceinline__ void sort_keys(unsigned (&key)[V]) {
 // A lane sorts its (up to 16) keys; each choice then costs one maximum over the token's lanes and one step down the winner's
 // list in shared memory, and which expert a winning key belongs to is looked up for all choices at once.  More keys than
 // that are searched again for every choice.
-// Bound by the instructions it issues, most of them the same for a token whatever its experts: 16 lanes to a token put two
-// tokens into each.
+// Bound by the integer instructions it issues (131072 x 256, top 8, fp32: about 550 a token, 117 to 132 us for what 22 would
+// read), many of them the same for a token whatever its experts: 16 lanes to a token put two tokens into each.  Keys
+// scanned again for every choice took 226 us, sorted together with their indices 140, ranked by pairs 120.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256)
 route_forward_kernel(const RouteArgs a) {
@@ -477,7 +478,8 @@ struct RouteBackwardArgs {
 //   normalised:  dl_e = [e in S] w_e (g_e - sum_S w g)          else:  dl_e = p_e ([e in S] g_e - sum_S p g)
 //   balance:     dl_e += db * E / tokens * p_e (f_e - sum_e' p_e' f_e')
 //   z:           dl_e += dz * 2 / tokens * lse * p_e
-// The softmax is formed again from the logits: reading them costs what reading a saved p would.
+// The softmax is formed again from the logits: reading them costs what reading a saved p would.  131072 x 256 fp32: 62 to
+// 74 us, 58 to 69 % of the copy rate; the chosen experts' own terms go through shared memory (by shuffles 77 us).
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256)
 route_backward_kernel(const RouteBackwardArgs a) {
@@ -548,6 +550,7 @@ route_backward_kernel(const RouteBackwardArgs a) {
 // Every block owns `chunk` consecutive choices, every warp of it an equal consecutive part.  A block's first row for an
 // expert is what earlier experts hold altogether plus what earlier blocks hold of this one: every block adds up all
 // histograms (they stay in the second-level cache), which costs less than a third launch that would do it once.
+// Bound by latency: 131072 x 8 choices of 256 experts 20 us, 32768 x 4 of 128 10 us (a thread per four experts: 45 and 14).
 __device__ __forceinline__ int read_choice(const void* indices, int is_long, long long i, int experts) {
   const long long e = is_long ? reinterpret_cast<const long long*>(indices)[i] : (long long)reinterpret_cast<const int*>(indices)[i];
   return e >= 0 && e < experts ? (int)e : -1;
@@ -663,7 +666,8 @@ __device__ __forceinline__ void clear_tail(W* rows, long long words, long long f
     for (long long c = threadIdx.x & 31; c < words; c += 32) rows[r * words + c] = W{};
 }
 
-// One warp per (token, segment of 32 * U words): the token's words are read once and stored top_k times.
+// One warp per (token, segment of 32 * U words): the token's words are read once and stored top_k times.  Bound by memory:
+// 32768 x 2048 bf16 to four experts 107 us, 96 % of the copy rate.
 template <typename W, int U>
 __global__ void __launch_bounds__(256)
 dispatch_kernel(const W* __restrict__ x, long long x_words, int words, int segments, int tokens, int top_k,
@@ -713,7 +717,9 @@ template <typename T, int N> struct Pack {       // N values of T moved as one w
   }
 };
 
-// out[t] = sum_j weights[t, j] * rows[positions[t, j]], added in fp32 in the order of j; weights null: all one
+// out[t] = sum_j weights[t, j] * rows[positions[t, j]], added in fp32 in the order of j; weights null: all one.
+// A warp per (token, segment of 32 * U packs).  Bound by memory: 32768 x 2048 bf16, four choices, 106 us (97 % of the copy
+// rate); threads over the flattened result instead of warps over rows took 158.
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(256)
 combine_kernel(const T* __restrict__ rows, int width, int segments, int tokens, int top_k, const int* __restrict__ positions,
