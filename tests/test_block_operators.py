@@ -606,7 +606,8 @@ def test_norm_refusals(device):
     x, w = torch.zeros(2, 3, 32, device=device), torch.ones(32, device=device)
     for bad in (dict(weight=w[:31]), dict(weight=torch.ones(2, 32, device=device)), dict(gate=torch.ones(3, 32, device=device)),
                 dict(gate=torch.ones(2, 3, 32, device=device)), dict(next_weight=w), dict(next_scale=w), dict(eps=0.0),
-                dict(eps=math.nan), dict(residual_scale=math.inf), dict(residual_scale=w)):
+                dict(eps=math.nan), dict(eps=1e-60), dict(eps=math.inf), dict(residual_scale=math.inf), dict(residual_scale=math.nan),
+                dict(residual_scale=-1e39), dict(residual_scale=w)):
         with pytest.raises(ValueError):
             nn.rms_norm_residual(x, x, **bad)
     for bad in (lambda: nn.rms_norm_residual(x, x[:1]), lambda: nn.rms_norm_modulate(torch.zeros(2, 16385, device=device)),

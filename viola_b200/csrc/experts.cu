@@ -168,11 +168,12 @@ template <int V> __device__ __forceinline__ void sort_keys(unsigned (&key)[V]) {
 // A lane sorts its (up to 16) keys; each choice then costs one maximum over the token's lanes and one step down the winner's
 // list in shared memory, and which expert a winning key belongs to is looked up for all choices at once.  More keys than
 // that are searched again for every choice.
-// Bound by the integer instructions it issues (131072 x 256, top 8, fp32: about 550 a token, 117 to 132 us for what 22 would
+// Bound by the integer instructions it issues (131072 x 256, top 8, fp32: about 550 a token, 119 us for what 22 would
 // read), many of them the same for a token whatever its experts: 16 lanes to a token put two tokens into each.  Keys
 // scanned again for every choice took 226 us, sorted together with their indices 140, ranked by pairs 120.
+// Four blocks an SM: 64 registers hold 16 keys a lane, and 32 warps hide the exchanges (119 us; 139 with 105 registers).
 template <typename T, int G, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, V <= 16 ? 4 : 2)
 route_forward_kernel(const RouteArgs a) {
   constexpr int kWarps = 8, kThreads = kWarps * 32;
   constexpr int kTokens = 32 / G;               // tokens a warp serves at a time
@@ -478,10 +479,10 @@ struct RouteBackwardArgs {
 //   normalised:  dl_e = [e in S] w_e (g_e - sum_S w g)          else:  dl_e = p_e ([e in S] g_e - sum_S p g)
 //   balance:     dl_e += db * E / tokens * p_e (f_e - sum_e' p_e' f_e')
 //   z:           dl_e += dz * 2 / tokens * lse * p_e
-// The softmax is formed again from the logits: reading them costs what reading a saved p would.  131072 x 256 fp32: 62 to
-// 74 us, 58 to 69 % of the copy rate; the chosen experts' own terms go through shared memory (by shuffles 77 us).
+// The softmax is formed again from the logits: reading them costs what reading a saved p would.  131072 x 256 fp32: 70 us,
+// 61 % of the copy rate (80 at two blocks an SM); the chosen experts' own terms go through shared memory (by shuffles 77 us).
 template <typename T, int G, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, V <= 16 ? 4 : 2)
 route_backward_kernel(const RouteBackwardArgs a) {
   constexpr int kTokens = 32 / G;
   __shared__ float chosen_grad[8][32 * V];      // of the tokens that a warp works on, zero where not chosen
@@ -721,7 +722,7 @@ template <typename T, int N> struct Pack {       // N values of T moved as one w
 // A warp per (token, segment of 32 * U packs).  Bound by memory: 32768 x 2048 bf16, four choices, 106 us (97 % of the copy
 // rate); threads over the flattened result instead of warps over rows took 158.
 template <typename T, int N, int U>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 combine_kernel(const T* __restrict__ rows, int width, int segments, int tokens, int top_k, const int* __restrict__ positions,
                const void* __restrict__ weights, int weight_dtype, T* __restrict__ out) {
   const int lane = threadIdx.x & 31;
@@ -762,9 +763,10 @@ combine_kernel(const T* __restrict__ rows, int width, int segments, int tokens, 
 // drows[positions[t, j]] = weights[t, j] * dout[t],  dweights[t, j] = <dout[t], rows[positions[t, j]]>
 // A token is served by `team` warps of a block (1, 2, 4 or 8) with up to U packs a lane in flight; after the first choice
 // its row of dout comes from the cache, and the dot products end in the block.
-// 32768 tokens x 1152 bf16, two choices: 94 us with two warps of four packs that split a row unevenly, 77 us evenly.
+// 32768 tokens x 1152 bf16, two choices: 94 us with two warps of four packs that split a row unevenly, 77 us evenly, 67 us
+// with one warp of five (82 % of the copy rate).  Bound by loads in flight: at 2 blocks an SM instead of 3 or 4 it takes 109.
 template <typename T, int N, int U>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, U <= 4 ? 4 : 3)
 combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, int width, int tokens, int top_k, int team,
                         const int* __restrict__ positions, const int* __restrict__ offsets, int experts,
                         const void* __restrict__ weights, int weight_dtype, T* __restrict__ drows, void* __restrict__ dweights) {
@@ -1020,7 +1022,7 @@ extern "C" int vb_expert_combine_backward(const void* dout, const void* rows, in
   if (tokens == 0) return 0;
   const int size = dtype == kF32 ? 4 : 2, pack = 16 / size;
   const bool wide = width % pack == 0 && aligned_to(rows, 16) && aligned_to(dout, 16) && (drows == nullptr || aligned_to(drows, 16));
-  // (at most 5 packs a lane: 32768 x 2048 bf16, four choices, 195 us with two warps a token, 204 to 249 with one of 8 packs)
+  // (at most 5 packs a lane: 32768 x 2048 bf16, four choices, 199 us with two warps of four, 249 with one of eight)
   const int packs = wide ? width / pack : width, most = std::min(5, row_packs(packs, tokens));
   int team = 1;
   while (team < 8 && packs > team * 32 * most) team *= 2;

@@ -10,12 +10,11 @@ follows it: the block's result ``y`` is normalised, gated and added to the scale
 Each call is one kernel forward and one (plus a small one for the gradients of the vectors) backward; nothing but two
 numbers per row is kept besides the inputs.  Vectors are [width] (shared by all rows) or [batch, width] with
 ``x`` [batch, ..., width] (one per sample, as an adaLN projection gives them).  CPU tensors take the same path through
-the PyTorch restatement.
+the PyTorch restatement.  On the GPU the gradients cannot be differentiated again.
 """
 
 from __future__ import annotations
 
-import math
 from numbers import Real
 
 import torch
@@ -23,6 +22,7 @@ import torch
 from .. import ops
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+_FP32 = torch.finfo(torch.float32)
 
 
 def _vector(v, x, name, samples=True):
@@ -48,8 +48,8 @@ def _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dt
         raise ValueError(f"the width must be between 1 and {ops.MAX_NORM_WIDTH}, got x of shape {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if not (isinstance(eps, Real) and eps > 0 and math.isfinite(eps)):
-        raise ValueError(f"eps must be a positive number, got {eps}")
+    if not (isinstance(eps, Real) and _FP32.tiny <= eps <= _FP32.max):
+        raise ValueError(f"eps must be a positive fp32 number, got {eps}")
     _vector(weight, x, "weight", samples=False)
     _vector(next_weight, x, "weight" if y is None else "next_weight", samples=False)
     per_sample = _vector(gate, x, "gate")
@@ -94,8 +94,8 @@ def rms_norm_residual(x, y, weight=None, gate=None, *, residual_scale=1.0, eps=1
         raise TypeError(f"x must be float32 or have the dtype of y, got {x.dtype} and {y.dtype}")
     if y.device != x.device:
         raise ValueError(f"y is on {y.device}, not on {x.device}")
-    if not (isinstance(residual_scale, Real) and math.isfinite(residual_scale)):
-        raise ValueError(f"residual_scale must be a finite number, got {residual_scale}")
+    if not (isinstance(residual_scale, Real) and abs(residual_scale) <= _FP32.max):
+        raise ValueError(f"residual_scale must be a finite fp32 number, got {residual_scale}")
     if not next_norm and (next_weight is not None or next_scale is not None):
         raise ValueError("next_weight and next_scale need next_norm=True")
     out, h = _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, y.dtype if next_norm else None)
