@@ -616,7 +616,8 @@ def test_norm_refusals(device):
         with pytest.raises(ValueError):
             bad()
     for bad in (lambda: nn.rms_norm_residual(x.half(), x), lambda: nn.rms_norm_residual(x.double(), x.double()),
-                lambda: nn.rms_norm_residual(x, x.double()), lambda: nn.rms_norm_residual(x, x, w.double()),
+                lambda: nn.rms_norm_residual(x, x.double()), lambda: nn.rms_norm_residual(x, x.double(), next_norm=True),
+                lambda: nn.rms_norm_residual(x, x, w.double()),
                 lambda: nn.rms_norm_modulate(x.half(), dtype=FP32), lambda: nn.rms_norm_modulate(x, dtype=torch.float64)):
         with pytest.raises(TypeError):
             bad()

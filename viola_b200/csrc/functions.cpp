@@ -4,13 +4,17 @@
 // nodes of their own, written in C++: calls on a few tokens are bound by the host, where a step through Python nodes and
 // Python allocations took 115 to 210 us.  A workspace belongs to one call (the caching allocator's, or the capture's
 // pool), so neither streams nor captured graphs share one.
-// Argument checks with the caller's names are in viola_b200/nn; those here guard the pointers.
+// Arguments are checked here too (ValueError, TypeError): in Python the checks of a call took as long as its launch.  The
+// same rules for CPU tensors are in viola_b200/nn.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
+#include <algorithm>
 #include <atomic>
+#include <cmath>
+#include <limits>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -23,12 +27,14 @@ using OptTensor = std::optional<Tensor>;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32, kMaxWidth = 1 << 22;
+
 std::atomic<int64_t> launches{0};     // kernels launched from here (bench bookkeeping)
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 int dtype_code(at::ScalarType t) {
-  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "viola_b200: expected float32, bfloat16 or float16, got ", t);
+  TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "expected float32, bfloat16 or float16, got ", t);
   return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2;
 }
 void check(int rc, const char* what, int kernels) {
@@ -36,7 +42,7 @@ void check(int rc, const char* what, int kernels) {
   launches.fetch_add(kernels, std::memory_order_relaxed);
 }
 int narrow(int64_t v, const char* name) {
-  TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, "viola_b200: ", name, " out of range: ", v);
+  TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " out of range: ", v);
   return (int)v;
 }
 void once_only() {
@@ -52,7 +58,7 @@ const Tensor& value(const OptTensor& t) { return t.has_value() ? *t : none(); }
 void* ptr(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 // a CUDA tensor on the device of `like` with unit column stride, as [rows, last dimension]
 void on_device(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK_VALUE(t.device() == like.device() && t.is_cuda(), "viola_b200: ", name, " must be on ", like.device());
+  TORCH_CHECK_VALUE(t.device() == like.device() && t.is_cuda(), name, " is on ", t.device(), ", not on ", like.device());
 }
 Tensor rows2d(const Tensor& t) {
   Tensor flat = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
@@ -70,20 +76,27 @@ struct Routed {
 };
 
 Routed route_forward(const Tensor& logits, int64_t top_k, const OptTensor& bias, const OptTensor& mask, bool normalize, bool save) {
-  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1, "viola_b200: logits must be a CUDA tensor [..., experts]");
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() >= 1, "logits must be a CUDA tensor with an experts dimension");
   const c10::cuda::CUDAGuard guard(logits.device());
   Routed r;
-  const int experts = narrow(logits.size(-1), "experts");
-  TORCH_CHECK_VALUE(experts > 0, "viola_b200: no experts");
-  const int tokens = narrow(logits.numel() / experts, "tokens"), dtype = dtype_code(logits.scalar_type());
+  const int64_t experts = logits.size(-1);
+  const int dtype = dtype_code(logits.scalar_type());
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, "the number of experts must be between 1 and ", kMaxExperts, ", got ", experts);
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= std::min(experts, kMaxTopK), "top_k must be between 1 and min(experts, ", kMaxTopK,
+                    "), got ", top_k, " for ", experts, " experts");
+  const int tokens = narrow(logits.numel() / experts, "tokens");
   r.flat = tokens > 0 ? rows2d(logits) : logits.reshape({0, experts});
+  Tensor offsets, live;
   if (bias.has_value()) {
     on_device(*bias, logits, "bias");
-    TORCH_CHECK_VALUE(bias->is_contiguous() && bias->scalar_type() == at::kFloat && bias->numel() == experts, "viola_b200: bias");
+    TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == experts, "bias must have shape (", experts, ",), got ", bias->sizes());
+    offsets = bias->detach().to(at::kFloat).contiguous();
   }
   if (mask.has_value()) {
     on_device(*mask, logits, "mask");
-    TORCH_CHECK_VALUE(mask->is_contiguous() && mask->scalar_type() == at::kBool && mask->numel() == tokens, "viola_b200: mask");
+    TORCH_CHECK_VALUE(mask->scalar_type() == at::kBool && mask->sizes() == logits.sizes().slice(0, logits.dim() - 1),
+                      "mask must be bool of the leading shape of logits ", logits.sizes(), ", got ", mask->scalar_type(), " ", mask->sizes());
+    live = mask->contiguous();
   }
   const auto f32 = logits.options().dtype(at::kFloat), i32 = logits.options().dtype(at::kInt);
   const at::DimVector shape = with_last(logits.sizes(), top_k);
@@ -96,8 +109,8 @@ Routed route_forward(const Tensor& logits, int64_t top_k, const OptTensor& bias,
   const Tensor scratch = at::empty({need + (save ? 0 : 2)}, f32);
   if (save) r.inverse = at::empty({2}, f32);
   float* work = scratch.data_ptr<float>();
-  check(vb_route_forward(r.flat.data_ptr(), dtype, tokens, experts, r.flat.stride(0), (const float*)ptr(value(bias)),
-                         (const uint8_t*)ptr(value(mask)), (int)top_k, normalize, r.weights.data_ptr<float>(),
+  check(vb_route_forward(r.flat.data_ptr(), dtype, tokens, (int)experts, r.flat.stride(0), (const float*)ptr(offsets),
+                         (const uint8_t*)ptr(live), (int)top_k, normalize, r.weights.data_ptr<float>(),
                          r.indices.data_ptr<int>(), r.counts.data_ptr<int>(), r.balance.data_ptr<float>(),
                          r.z.data_ptr<float>(), save ? r.inverse.data_ptr<float>() : work + need, work, need, stream()),
         "route_forward", 1);
@@ -148,8 +161,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor& logits, i
 
 // ---- plan, dispatch, combine -------------------------------------------------------------------------------------
 std::tuple<Tensor, Tensor> expert_plan(const Tensor& indices, int64_t experts) {
-  TORCH_CHECK_TYPE(indices.scalar_type() == at::kInt || indices.scalar_type() == at::kLong, "viola_b200: indices must be int32 or int64");
-  TORCH_CHECK_VALUE(indices.is_cuda() && indices.dim() >= 1 && indices.size(-1) >= 1, "viola_b200: indices must be a CUDA tensor [..., top_k]");
+  TORCH_CHECK_TYPE(indices.dim() >= 1 && (indices.scalar_type() == at::kInt || indices.scalar_type() == at::kLong),
+                   "indices must be int32 or int64 [..., top_k], got ", indices.scalar_type(), " ", indices.sizes());
+  TORCH_CHECK_VALUE(indices.is_cuda(), "indices must be a CUDA tensor");
+  TORCH_CHECK_VALUE(experts >= 1 && experts <= kMaxExperts, "the number of experts must be between 1 and ", kMaxExperts, ", got ", experts);
+  TORCH_CHECK_VALUE(indices.size(-1) >= 1 && indices.size(-1) <= kMaxTopK, "indices must hold between 1 and ", kMaxTopK,
+                    " choices per token, got ", indices.size(-1));
   const c10::cuda::CUDAGuard guard(indices.device());
   const Tensor flat = indices.contiguous();
   const int n = narrow(flat.numel(), "choices"), e = narrow(experts, "experts");
@@ -165,14 +182,16 @@ std::tuple<Tensor, Tensor> expert_plan(const Tensor& indices, int64_t experts) {
 
 struct Plan {
   int tokens, top_k, experts;
+  Tensor positions, offsets;
 };
 Plan check_plan(const Tensor& positions, const Tensor& offsets, const Tensor& like) {
   on_device(positions, like, "positions");
   on_device(offsets, like, "offsets");
-  TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt && positions.dim() == 2 && positions.is_contiguous() &&
-                    offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.is_contiguous() && offsets.numel() >= 2,
-                    "viola_b200: a plan holds contiguous int32 offsets [experts + 1] and positions [tokens, top_k]");
-  return {narrow(positions.size(0), "tokens"), narrow(positions.size(1), "top_k"), (int)offsets.numel() - 1};
+  TORCH_CHECK_VALUE(positions.scalar_type() == at::kInt && positions.dim() == 2 && positions.size(1) >= 1 &&
+                    positions.size(1) <= kMaxTopK && offsets.scalar_type() == at::kInt && offsets.dim() == 1 && offsets.numel() >= 2,
+                    "plan must hold int32 offsets [experts + 1] and int32 positions [tokens, top_k]");
+  narrow(positions.numel(), "choices");
+  return {(int)positions.size(0), (int)positions.size(1), narrow(offsets.numel(), "experts") - 1, positions.contiguous(), offsets.contiguous()};
 }
 
 Tensor combine_forward(const Tensor& rows, const Tensor& weights, const Tensor& positions, at::IntArrayRef shape) {
@@ -184,10 +203,11 @@ Tensor combine_forward(const Tensor& rows, const Tensor& weights, const Tensor& 
   return out;
 }
 
-Tensor dispatch_forward(const Tensor& x, const Tensor& positions, const Tensor& offsets) {
-  const Plan plan = check_plan(positions, offsets, x);
+Tensor dispatch_forward(const Tensor& x, const Plan& plan) {
+  const Tensor &positions = plan.positions, &offsets = plan.offsets;
   dtype_code(x.scalar_type());
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.numel() == plan.tokens * x.size(-1), "viola_b200: x does not hold the plan's tokens");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= kMaxWidth && x.numel() == plan.tokens * x.size(-1),
+                    "x of shape ", x.sizes(), " does not hold the plan's ", plan.tokens, " tokens");
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t width = x.size(-1);
   const Tensor flat = plan.tokens ? rows2d(x) : x.reshape({0, width});
@@ -200,9 +220,10 @@ Tensor dispatch_forward(const Tensor& x, const Tensor& positions, const Tensor& 
 
 struct Dispatch : torch::autograd::Function<Dispatch> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& positions, const Tensor& offsets) {
-    ctx->save_for_backward({positions});
+    const Plan plan = check_plan(positions, offsets, x);
+    ctx->save_for_backward({plan.positions});
     ctx->saved_data["shape"] = x.sizes().vec();
-    return dispatch_forward(x, positions, offsets);
+    return dispatch_forward(x, plan);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
@@ -214,16 +235,19 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
 
 Tensor expert_dispatch(const Tensor& x, const Tensor& positions, const Tensor& offsets) {
   if (at::GradMode::is_enabled() && wants_grad(x)) return Dispatch::apply(x, positions, offsets);
-  return dispatch_forward(x, positions, offsets);
+  return dispatch_forward(x, check_plan(positions, offsets, x));
 }
 
-void check_combine(const Tensor& rows, const Tensor& weights, const Tensor& positions, const Tensor& offsets) {
+Plan check_combine(const Tensor& rows, const Tensor& weights, const Tensor& positions, const Tensor& offsets) {
   const Plan plan = check_plan(positions, offsets, rows);
   on_device(weights, rows, "weights");
+  dtype_code(rows.scalar_type());
   dtype_code(weights.scalar_type());
-  TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == positions.numel() && rows.size(1) >= 1 && weights.dim() >= 1 &&
-                    weights.size(-1) == plan.top_k && weights.numel() == positions.numel(),
-                    "viola_b200: rows and weights do not match the plan");
+  TORCH_CHECK_VALUE(rows.dim() == 2 && rows.size(0) == positions.numel() && rows.size(1) >= 1 && rows.size(1) <= kMaxWidth,
+                    "rows must be [", positions.numel(), ", width], got ", rows.sizes());
+  TORCH_CHECK_VALUE(weights.dim() >= 1 && weights.size(-1) == plan.top_k && weights.numel() == positions.numel(),
+                    "weights of shape ", weights.sizes(), " do not match the plan's ", plan.tokens, " tokens x ", plan.top_k, " choices");
+  return plan;
 }
 
 struct Combine : torch::autograd::Function<Combine> {
@@ -252,21 +276,23 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 Tensor expert_combine(const Tensor& rows, const Tensor& weights, const Tensor& positions, const Tensor& offsets) {
-  check_combine(rows, weights, positions, offsets);
+  const Plan plan = check_combine(rows, weights, positions, offsets);
   if (at::GradMode::is_enabled() && (wants_grad(rows) || wants_grad(weights)))
-    return Combine::apply(rows, weights, positions, offsets);
+    return Combine::apply(rows, weights, plan.positions, plan.offsets);
   const c10::cuda::CUDAGuard guard(rows.device());
-  return combine_forward(rows.contiguous(), weights.contiguous(), positions, with_last(weights.sizes(), rows.size(1)));
+  return combine_forward(rows.contiguous(), weights.contiguous(), plan.positions, with_last(weights.sizes(), rows.size(1)));
 }
 
 // ---- RMS norms around a block --------------------------------------------------------------------------------------
-// [cols]: shared by all rows; [samples, cols]: one row per sample; anything the kernels cannot read in place is copied
-Tensor vector_in_place(const OptTensor& t, const Tensor& x, int64_t samples, const char* name) {
+// [cols]: shared by all rows; [batch, cols] where `samples`: one row per sample; what the kernels cannot read in place is copied
+Tensor vector_in_place(const OptTensor& t, const Tensor& x, bool samples, const char* name) {
   if (!t.has_value()) return Tensor();
   on_device(*t, x, name);
   dtype_code(t->scalar_type());
   const int64_t cols = x.size(-1);
-  TORCH_CHECK_VALUE((t->dim() == 1 || (t->dim() == 2 && t->size(0) == samples)) && t->size(-1) == cols, "viola_b200: shape of ", name);
+  const bool per_sample = samples && x.dim() >= 2 && t->dim() == 2 && t->size(0) == x.size(0) && t->size(1) == cols;
+  TORCH_CHECK_VALUE(per_sample || (t->dim() == 1 && t->size(0) == cols), name, " must have shape (", cols, ",)",
+                    samples ? " or (batch, width)" : "", " for x of shape ", x.sizes(), ", got ", t->sizes());
   const bool rows_apart = t->dim() == 1 || t->size(0) == 1 || t->stride(0) >= cols;
   return (t->stride(-1) == 1 || cols == 1) && rows_apart ? *t : t->contiguous();
 }
@@ -278,6 +304,7 @@ VbNormVector norm_vector(const Tensor& t) {
 
 struct Normed {
   Tensor x, y, weight, gate, next_weight, next_scale, out, h, ry, ru;
+  int64_t tokens = 0;
   VbBlockNorm args{};
 };
 
@@ -301,33 +328,42 @@ VbBlockNorm norm_args(const Normed& n, int64_t rows, int64_t cols, int64_t token
   return a;
 }
 
-// h_dtype: -1 for no h, else a dtype code; tokens: rows of a sample (all rows where no vector is per sample)
+// h_dtype: -1 for no h, else a dtype code
 Normed norm_forward(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate, const OptTensor& next_weight,
-                    const OptTensor& next_scale, int64_t tokens, double residual_scale, double eps, int64_t h_dtype, bool save) {
-  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.numel() > 0 && tokens >= 1, "viola_b200: x must be a CUDA tensor with rows");
+                    const OptTensor& next_scale, double residual_scale, double eps, int64_t h_dtype, bool save) {
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.numel() > 0 && x.size(-1) <= VB_NORM_MAX_COLS,
+                    "the width must be between 1 and ", VB_NORM_MAX_COLS, ", got x of shape ", x.sizes());
+  dtype_code(x.scalar_type());
+  constexpr double most = std::numeric_limits<float>::max(), least = std::numeric_limits<float>::min();
+  TORCH_CHECK_VALUE(eps >= least && eps <= most, "eps must be a positive fp32 number, got ", eps);
+  TORCH_CHECK_VALUE(std::abs(residual_scale) <= most, "residual_scale must be a finite fp32 number, got ", residual_scale);
   const c10::cuda::CUDAGuard guard(x.device());
   const int64_t cols = x.size(-1), rows = x.numel() / cols;
-  TORCH_CHECK_VALUE(rows % tokens == 0, "viola_b200: rows must be whole samples");
   Normed n;
   n.x = x.contiguous();
   if (y.has_value()) {
     on_device(*y, x, "y");
-    TORCH_CHECK_VALUE(y->sizes() == x.sizes(), "viola_b200: y must have the shape of x");
+    TORCH_CHECK_VALUE(y->sizes() == x.sizes(), "y must have the shape of x, got ", y->sizes(), " and ", x.sizes());
+    dtype_code(y->scalar_type());
+    TORCH_CHECK_TYPE(x.scalar_type() == at::kFloat || x.scalar_type() == y->scalar_type(),
+                     "x must be float32 or have the dtype of y, got ", x.scalar_type(), " and ", y->scalar_type());
     n.y = y->contiguous();
     n.out = at::empty(x.sizes(), x.options());
   }
-  const int64_t samples = rows / tokens;
-  n.weight = vector_in_place(weight, x, samples, "weight");
-  n.gate = vector_in_place(gate, x, samples, "gate");
-  n.next_weight = vector_in_place(next_weight, x, samples, "next_weight");
-  n.next_scale = vector_in_place(next_scale, x, samples, "next_scale");
+  n.weight = vector_in_place(weight, x, false, "weight");
+  n.gate = vector_in_place(gate, x, true, "gate");
+  n.next_weight = vector_in_place(next_weight, x, false, y.has_value() ? "next_weight" : "weight");
+  n.next_scale = vector_in_place(next_scale, x, true, y.has_value() ? "next_scale" : "scale");
+  // rows of a sample (all rows where no vector is per sample)
+  const bool per_sample = (n.gate.defined() && n.gate.dim() == 2) || (n.next_scale.defined() && n.next_scale.dim() == 2);
+  n.tokens = per_sample ? rows / x.size(0) : rows;
   const auto f32 = x.options().dtype(at::kFloat);
   if (h_dtype >= 0) n.h = at::empty(x.sizes(), x.options().dtype(h_dtype == 0 ? at::kFloat : h_dtype == 1 ? at::kBFloat16 : at::kHalf));
   if (save && n.y.defined()) n.ry = at::empty({rows}, f32);
   if (save && n.h.defined()) n.ru = at::empty({rows}, f32);
   const int y_dtype = n.y.defined() ? dtype_code(n.y.scalar_type()) : (int)h_dtype;
   TORCH_CHECK_TYPE(h_dtype < 0 || h_dtype == y_dtype, "viola_b200: h has the dtype of y");
-  n.args = norm_args(n, rows, cols, tokens, residual_scale, eps, y_dtype);
+  n.args = norm_args(n, rows, cols, n.tokens, residual_scale, eps, y_dtype);
   n.args.out = ptr(n.out);
   n.args.h = ptr(n.h);
   check(vb_block_norm(&n.args, stream()), "block_norm", 1);
@@ -342,11 +378,11 @@ variable_list norm_results(const Normed& n) {
 
 struct BlockNorm : torch::autograd::Function<BlockNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& y, const OptTensor& weight,
-                               const OptTensor& gate, const OptTensor& next_weight, const OptTensor& next_scale, int64_t tokens,
+                               const OptTensor& gate, const OptTensor& next_weight, const OptTensor& next_scale,
                                double residual_scale, double eps, int64_t h_dtype) {
-    const Normed n = norm_forward(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype, true);
+    const Normed n = norm_forward(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype, true);
     ctx->save_for_backward({n.x, n.y, n.weight, n.gate, n.next_weight, n.next_scale, n.ry, n.ru});
-    ctx->saved_data["tokens"] = tokens;
+    ctx->saved_data["tokens"] = n.tokens;
     ctx->saved_data["residual_scale"] = residual_scale;
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["y_dtype"] = (int64_t)n.args.y_dtype;
@@ -356,7 +392,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     once_only();
-    variable_list result(10);
+    variable_list result(9);
     const variable_list saved = ctx->get_saved_variables();
     Normed n;
     n.x = saved[0]; n.y = saved[1]; n.weight = saved[2]; n.gate = saved[3];
@@ -398,12 +434,12 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 };
 
 std::vector<Tensor> block_norm(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate,
-                               const OptTensor& next_weight, const OptTensor& next_scale, int64_t tokens, double residual_scale,
-                               double eps, int64_t h_dtype) {
+                               const OptTensor& next_weight, const OptTensor& next_scale, double residual_scale, double eps,
+                               int64_t h_dtype) {
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(y) || wants_grad(weight) || wants_grad(gate) ||
                                      wants_grad(next_weight) || wants_grad(next_scale)))
-    return BlockNorm::apply(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype);
-  return norm_results(norm_forward(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype, false));
+    return BlockNorm::apply(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype);
+  return norm_results(norm_forward(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype, false));
 }
 
 int64_t block_launches() { return launches.load(std::memory_order_relaxed); }

@@ -23,7 +23,6 @@ import torch
 from .. import ops
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_MAX_WIDTH = 1 << 22
 
 
 class Routing(NamedTuple):
@@ -64,6 +63,8 @@ def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
 
     ``balance_loss = experts * sum_e f_e P_e`` with f_e the expert's share of all choices (``counts``) and P_e the mean of
     its p; ``z_loss`` is the mean squared log-sum-exp.  Gradients of the weights and of both losses reach ``logits``."""
+    if logits.is_cuda:                       # checked by the operator
+        return Routing(*ops.route(logits, top_k, bias=bias, mask=mask, normalize=normalize))
     if logits.dim() < 1:
         raise ValueError("logits must have an experts dimension")
     _float(logits, "logits")
@@ -88,6 +89,8 @@ def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
 def plan_experts(indices, num_experts):
     """Where the choices ``indices`` (int32 or int64 [..., top_k]) go when sorted by expert, tokens in order within an
     expert.  Values outside ``0 .. num_experts - 1`` are dropped: they take no row."""
+    if indices.is_cuda:
+        return ExpertPlan(*ops.expert_plan(indices, num_experts))
     if indices.dim() < 1 or indices.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"indices must be int32 or int64 [..., top_k], got {indices.dtype} {tuple(indices.shape)}")
     if not 1 <= num_experts <= ops.MAX_EXPERTS:
@@ -112,10 +115,12 @@ def _check_plan(plan, tensor, name):
 def dispatch_tokens(x, plan):
     """The rows of ``x`` [..., width] sorted by expert: [tokens * top_k, width], one row per choice, zeros behind the last
     expert's rows (``plan.offsets[-1]``)."""
+    if x.is_cuda:
+        return ops.expert_dispatch(x, plan[1], plan[0])
     offsets, positions = _check_plan(plan, x, "x")
     _float(x, "x")
     width = x.shape[-1]
-    if not 1 <= width <= _MAX_WIDTH or x.numel() != positions.shape[0] * width:
+    if not 1 <= width <= ops.MAX_DISPATCH_WIDTH or x.numel() != positions.shape[0] * width:
         raise ValueError(f"x of shape {tuple(x.shape)} does not hold the plan's {positions.shape[0]} tokens")
     return ops.expert_dispatch(x, positions, offsets)
 
@@ -126,12 +131,14 @@ def combine_tokens(rows, weights, plan):
     ``rows`` [tokens * top_k, width] as :func:`dispatch_tokens` lays them out, ``weights`` [..., top_k] (float32, bfloat16
     or float16).  A choice without a row adds nothing; rows behind the last expert's are not read, and their gradient is
     zero.  Sums are taken in fp32 and rounded once to the rows' dtype."""
+    if rows.is_cuda:
+        return ops.expert_combine(rows, weights, plan[1], plan[0])
     offsets, positions = _check_plan(plan, rows, "rows")
     _float(rows, "rows")
     _float(weights, "weights")
     _same_device(weights, "weights", rows)
     tokens, top_k = positions.shape
-    if rows.dim() != 2 or rows.shape[0] != tokens * top_k or not 1 <= rows.shape[1] <= _MAX_WIDTH:
+    if rows.dim() != 2 or rows.shape[0] != tokens * top_k or not 1 <= rows.shape[1] <= ops.MAX_DISPATCH_WIDTH:
         raise ValueError(f"rows must be [{tokens * top_k}, width], got {tuple(rows.shape)}")
     if weights.dim() < 1 or weights.shape[-1] != top_k or weights.numel() != tokens * top_k:
         raise ValueError(f"weights of shape {tuple(weights.shape)} do not match the plan's {tokens} tokens x {top_k} choices")

@@ -26,44 +26,51 @@ _FP32 = torch.finfo(torch.float32)
 
 
 def _vector(v, x, name, samples=True):
-    """Check an optional vector; returns whether it has one row per sample."""
+    """Check an optional vector: [width], or with ``samples`` [batch, width]."""
     if v is None:
-        return False
+        return
     if v.dtype not in _DTYPES:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {v.dtype}")
     if v.device != x.device:
         raise ValueError(f"{name} is on {v.device}, not on {x.device}")
     width = x.shape[-1]
-    if v.shape == (width,):
-        return False
-    if samples and x.dim() >= 2 and v.shape == (x.shape[0], width):
-        return True
+    if v.shape == (width,) or (samples and x.dim() >= 2 and v.shape == (x.shape[0], width)):
+        return
     shapes = f"({width},) or (batch, {width})" if samples else f"({width},)"
     raise ValueError(f"{name} must have shape {shapes} for x of shape {tuple(x.shape)}, got {tuple(v.shape)}")
 
 
 def _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype):
+    if not (type(residual_scale) is type(eps) is float or isinstance(residual_scale, Real) and isinstance(eps, Real)):
+        raise ValueError(f"residual_scale and eps must be numbers, got {type(residual_scale).__name__} and {type(eps).__name__}")
+    if x.is_cuda and x.numel():              # checked by the operator
+        return ops.block_norm(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype)
+    if y is not None:
+        if y.shape != x.shape:
+            raise ValueError(f"y must have the shape of x, got {tuple(y.shape)} and {tuple(x.shape)}")
+        if y.dtype not in _DTYPES or x.dtype not in (torch.float32, y.dtype):
+            raise TypeError(f"x must be float32 or have the dtype of y, got {x.dtype} and {y.dtype}")
+        if y.device != x.device:
+            raise ValueError(f"y is on {y.device}, not on {x.device}")
     width = x.shape[-1] if x.dim() else 0
     if not 1 <= width <= ops.MAX_NORM_WIDTH:
         raise ValueError(f"the width must be between 1 and {ops.MAX_NORM_WIDTH}, got x of shape {tuple(x.shape)}")
     if x.dtype not in _DTYPES:
         raise TypeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if not (isinstance(eps, Real) and _FP32.tiny <= eps <= _FP32.max):
+    if not _FP32.tiny <= eps <= _FP32.max:
         raise ValueError(f"eps must be a positive fp32 number, got {eps}")
+    if not abs(residual_scale) <= _FP32.max:
+        raise ValueError(f"residual_scale must be a finite fp32 number, got {residual_scale}")
     _vector(weight, x, "weight", samples=False)
     _vector(next_weight, x, "weight" if y is None else "next_weight", samples=False)
-    per_sample = _vector(gate, x, "gate")
-    per_sample |= _vector(next_scale, x, "scale" if y is None else "next_scale")
-    rows = x.numel() // width
+    _vector(gate, x, "gate")
+    _vector(next_scale, x, "scale" if y is None else "next_scale")
     inputs = (x, y, weight, gate, next_weight, next_scale)
-    if rows == 0:
+    if x.numel() == 0:
         # nothing to compute, but the graph reaches every input
         empty = sum(t.sum() * 0 for t in inputs if t is not None and t.requires_grad)
-        out = x + empty if y is not None else None
-        return out, (x + empty).to(h_dtype) if h_dtype is not None else None
-    tokens = rows // x.shape[0] if per_sample else rows
-    results = ops.block_norm(*inputs, tokens, float(residual_scale), float(eps), h_dtype)
-    return results[0] if y is not None else None, results[-1] if h_dtype is not None else None
+        return ([x + empty] if y is not None else []) + ([(x + empty).to(h_dtype)] if h_dtype is not None else [])
+    return ops.block_norm(*inputs, residual_scale, eps, h_dtype)
 
 
 def rms_norm_modulate(x, weight=None, scale=None, *, eps=1e-6, dtype=None):
@@ -77,7 +84,7 @@ def rms_norm_modulate(x, weight=None, scale=None, *, eps=1e-6, dtype=None):
             dtype = torch.get_autocast_dtype("cuda")
     if dtype not in _DTYPES or (x.dtype != torch.float32 and dtype != x.dtype):
         raise TypeError(f"cannot normalise {x.dtype} into {dtype}")
-    return _call(x, None, None, None, weight, scale, 1.0, eps, dtype)[1]
+    return _call(x, None, None, None, weight, scale, 1.0, eps, dtype)[0]
 
 
 def rms_norm_residual(x, y, weight=None, gate=None, *, residual_scale=1.0, eps=1e-6, next_norm=False, next_weight=None,
@@ -88,15 +95,7 @@ def rms_norm_residual(x, y, weight=None, gate=None, *, residual_scale=1.0, eps=1
     ``weight`` [width]; ``gate`` [width] or [batch, width].  With ``next_norm`` the result is ``(out, h)`` with
     ``h = out * (mean(out^2) + eps)^-1/2 * next_weight * (1 + next_scale)`` in the dtype of ``y``, taken from ``out`` before
     it is rounded: the input of the next block."""
-    if y.shape != x.shape:
-        raise ValueError(f"y must have the shape of x, got {tuple(y.shape)} and {tuple(x.shape)}")
-    if y.dtype not in _DTYPES or x.dtype not in (torch.float32, y.dtype):
-        raise TypeError(f"x must be float32 or have the dtype of y, got {x.dtype} and {y.dtype}")
-    if y.device != x.device:
-        raise ValueError(f"y is on {y.device}, not on {x.device}")
-    if not (isinstance(residual_scale, Real) and abs(residual_scale) <= _FP32.max):
-        raise ValueError(f"residual_scale must be a finite fp32 number, got {residual_scale}")
     if not next_norm and (next_weight is not None or next_scale is not None):
         raise ValueError("next_weight and next_scale need next_norm=True")
-    out, h = _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, y.dtype if next_norm else None)
-    return (out, h) if next_norm else out
+    results = _call(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, y.dtype if next_norm else None)
+    return tuple(results) if next_norm else results[0]

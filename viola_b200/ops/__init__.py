@@ -892,12 +892,20 @@ def gate_residual_backward(dout, gate, y, tokens, sums_dtype=torch.float32):
 # ------------------------------------------------------------------------------ expert routing
 # These operators and the norms below allocate their results and record their gradients in C++ (csrc/functions.cpp);
 # :func:`block_launches` counts the kernels launched there.  On the CPU autograd differentiates the restatements.
-MAX_EXPERTS, MAX_TOP_K = 1024, 32
+MAX_EXPERTS, MAX_TOP_K, MAX_DISPATCH_WIDTH = 1024, 32, 1 << 22
+_block_ops = {}
+
+
+def _block_op(name):
+    op = _block_ops.get(name)
+    if op is None:
+        op = _block_ops[name] = getattr(_ops(), name).default
+    return op
 
 
 def block_launches():
     """Kernels launched so far by the operators that record their own gradients."""
-    return _ops().block_launches()
+    return _block_op("block_launches")()
 
 
 def route(logits, top_k, *, bias=None, mask=None, normalize=True):
@@ -906,7 +914,7 @@ def route(logits, top_k, *, bias=None, mask=None, normalize=True):
     that have no key above -inf, get index -1 and weight 0 and enter no sum."""
     if not logits.is_cuda:
         return reference.route(logits, top_k, bias=bias, mask=mask, normalize=normalize)
-    return _ops().route(logits, top_k, bias, mask, normalize)
+    return _block_op("route")(logits, top_k, bias, mask, normalize)
 
 
 def expert_plan(indices, experts):
@@ -914,35 +922,37 @@ def expert_plan(indices, experts):
     (offsets int32 [experts + 1], positions int32 [tokens, top_k], -1 for a dropped choice)."""
     if not indices.is_cuda:
         return reference.expert_plan(indices, experts)
-    return _ops().expert_plan(indices, experts)
+    return _block_op("expert_plan")(indices, experts)
 
 
 def expert_dispatch(x, positions, offsets):
     """Rows sorted by expert: ``rows[positions[t, j]] = x[t]`` ([tokens * top_k, width]; rows behind the last are zero)."""
     if not x.is_cuda:
         return reference.expert_dispatch(x, positions, offsets)
-    return _ops().expert_dispatch(x, positions, offsets)
+    return _block_op("expert_dispatch")(x, positions, offsets)
 
 
 def expert_combine(rows, weights, positions, offsets):
     """``out[t] = sum_j weights[t, j] * rows[positions[t, j]]`` in fp32, rounded once."""
     if not rows.is_cuda:
         return reference.expert_combine(rows, weights, positions, offsets)
-    return _ops().expert_combine(rows, weights, positions, offsets)
+    return _block_op("expert_combine")(rows, weights, positions, offsets)
 
 
 # ------------------------------------------------------------------------------ RMS norms around a block
 MAX_NORM_WIDTH = 16384
 
 
-def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
+def block_norm(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype):
     """``out = residual_scale * x + gate * weight * rms(y)`` (with ``y``) and ``h = rms(out) * next_weight * (1 + next_scale)``
-    (with ``h_dtype``; ``out`` is ``x`` without ``y``) over the last dimension; the vectors are [width] or one row per
-    sample of ``tokens`` rows.  Returns those of (out, h) that were asked for."""
+    (with ``h_dtype``; ``out`` is ``x`` without ``y``) over the last dimension; the weights are [width], gate and
+    next_scale [width] or [batch, width].  Returns those of (out, h) that were asked for."""
     if not x.is_cuda:
-        return reference.block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype)
-    return _ops().block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps,
-                             -1 if h_dtype is None else _DT[h_dtype])
+        return reference.block_norm(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype)
+    code = -1 if h_dtype is None else _DT.get(h_dtype)
+    if code is None:
+        raise TypeError(f"expected float32, bfloat16 or float16, got {h_dtype}")
+    return _block_op("block_norm")(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, code)
 
 
 # ------------------------------------------------------------------------------ multi-tensor optimizer ops

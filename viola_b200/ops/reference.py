@@ -543,8 +543,10 @@ def expert_combine(rows, weights, positions, offsets):
 
 
 # --------------------------------------------------------------------------- RMS norms around a block
-def block_norm(x, y, weight, gate, next_weight, next_scale, tokens, residual_scale, eps, h_dtype):
+def block_norm(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype):
     width = x.shape[-1]
+    samples = x.shape[0] if any(v is not None and v.dim() == 2 for v in (gate, next_scale)) else 1
+    tokens = x.numel() // width // samples
 
     def factor(vector, shift=0.0):
         if vector is None:
