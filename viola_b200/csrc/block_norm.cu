@@ -132,7 +132,8 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // every thread, so few threads with many values each take the fewest instructions: as many as four pieces a thread, as long
 // as not more lanes idle for it (128 x 256 x 1152, fp32 stream: 120 us with one piece a thread, 86 with three; 4 x 8192 x 4096
 // bf16: 254 and 202).  Backward: a piece takes three times the registers, and warps to hide latency count for more
-// (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four).
+// (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four).  Shifted pieces
+// take more registers too: two a thread forward (4 x 4096 x 2047 bf16: 118 us with one, 103 with two, 133 with four).
 bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
   if (cols < 1 || cols > VB_NORM_MAX_COLS || (!shift && cols % kPiece)) return false;
   const int pieces = (cols + kPiece - 1) / kPiece;
@@ -141,7 +142,7 @@ bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
     s.v = pieces <= 512 ? 1 : pieces <= 1024 ? 2 : 4;
   } else {
     int best = INT_MAX;
-    for (int v = 4; v >= 1; --v) {
+    for (int v = shift && pieces <= 512 ? 2 : 4; v >= 1; --v) {
       const int warps = (pieces + 32 * v - 1) / (32 * v), cost = warps * (kPiece * v + 10);
       if (warps <= (v == 4 ? 16 : 8) && cost < best) {
         best = cost;
