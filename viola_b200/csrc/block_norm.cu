@@ -32,17 +32,22 @@ struct NormSumArgs {
 // Gradients of the vectors from what the row groups left.  The shared ones: with T the sum of the blocks' sums, T for a
 // weight whose partner is per sample (its factors are in T), partner * T for one whose partner is shared, and weight * T
 // for a shared partner.  Per-sample ones of samples that several groups shared: weight * sum of what they parked.
-// A block has 128 columns, 4 a thread, and 16 rows of threads: the first block of a column range (where anything is
-// shared) gives all of them to T, every other one eight to each of two samples, or of two group boundaries where there are
+// A block has one norm and 128 columns, 4 a thread, and 16 rows of threads: the first block of a column range (where anything
+// is shared) gives all of them to T, every other one eight to each of two samples, or of two group boundaries where there are
 // fewer of those; the first boundary inside a sample takes that sample.  A row takes every 16th (8th) set, and the rows are
-// added in order.
+// added in order.  What bounds it is the latency of the loads for T, one set of every block of the backward kernel (444 for
+// 128 x 256 x 1152), so a thread has eight under way.
 __global__ void __launch_bounds__(512)
 norm_sums_kernel(const NormSumArgs a) {
-  __shared__ float4 part[2][16][32];
-  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, c = blockIdx.y * 128 + lane * 4;
+  __shared__ float4 part[16][32];
+  const int lane = threadIdx.x & 31, row = threadIdx.x >> 5, c = blockIdx.y * 128 + lane * 4, n = blockIdx.z;
   const int has_shared = a.blocks > 0 ? 1 : 0;
   const bool shared_block = has_shared && blockIdx.x == 0;
   const int stride = shared_block ? 16 : 8, turn = shared_block ? row : row % 8;
+  const bool per_sample = a.partner[n].pitch != 0;
+  if (!(shared_block ? a.dweight[n] != nullptr || (a.dpartner[n] != nullptr && !per_sample)
+                     : a.dpartner[n] != nullptr && per_sample))
+    return;                                     // the whole block
   const float* from = a.sums;
   long long sample = 0, first = 0, last = a.blocks;
   if (!shared_block) {
@@ -68,41 +73,29 @@ norm_sums_kernel(const NormSumArgs a) {
       }
     }
   }
-  bool wanted[2];                               // the same for the whole block
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const bool per_sample = a.partner[n].pitch != 0;
-    wanted[n] = shared_block ? a.dweight[n] != nullptr || (a.dpartner[n] != nullptr && !per_sample)
-                             : a.dpartner[n] != nullptr && per_sample;
-  }
-  float total[2][4] = {};
-#pragma unroll 4
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
   for (long long u = first + turn; u < last; u += stride) {
     const long long set = shared_block ? u : u * 2 + (u > first ? 0 : 1);
+    if (c >= a.cols) continue;
+    const float* at = from + (set * 2 + n) * a.cols + c;
+    if (a.cols % 4 == 0) {
+      const float4 t = *reinterpret_cast<const float4*>(at);
+      total[0] += t.x; total[1] += t.y; total[2] += t.z; total[3] += t.w;
+    } else {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (!wanted[n] || c >= a.cols) continue;
-      const float* at = from + (set * 2 + n) * a.cols + c;
-      if (a.cols % 4 == 0) {
-        const float4 t = *reinterpret_cast<const float4*>(at);
-        total[n][0] += t.x; total[n][1] += t.y; total[n][2] += t.z; total[n][3] += t.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (c + i < a.cols) total[n][i] += at[i];
-      }
+      for (int i = 0; i < 4; ++i)
+        if (c + i < a.cols) total[i] += at[i];
     }
   }
-#pragma unroll
-  for (int n = 0; n < 2; ++n) part[n][row][lane] = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
+  part[row][lane] = make_float4(total[0], total[1], total[2], total[3]);
   __syncthreads();
-  // rows 0 and 1 of a set (two sets of eight, or one) finish one norm each
-  const int n = turn;
-  if (turn >= 2 || first >= last || !wanted[n]) return;
+  // the first row of a set (two sets of eight, or one) finishes it
+  if (turn > 0 || first >= last) return;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
-  for (int i = row - turn; i < row - turn + stride; ++i) {
-    const float4 t = part[n][i][lane];
+  for (int i = row; i < row + stride; ++i) {
+    const float4 t = part[i][lane];
     sum[0] += t.x; sum[1] += t.y; sum[2] += t.z; sum[3] += t.w;
   }
   const NormVector &w = a.weight[n], &p = a.partner[n];
@@ -114,8 +107,8 @@ norm_sums_kernel(const NormSumArgs a) {
       store_from_float(a.dpartner[n], sample * a.cols + c + i, p.dtype, by_weight);
     } else {
       if (a.dweight[n] != nullptr)
-        store_from_float(a.dweight[n], c + i, w.dtype, p.pitch != 0 ? sum[i] : sum[i] * vector_value(p, 0, c + i, n ? 1.f : 0.f, 1.f));
-      if (a.dpartner[n] != nullptr && p.pitch == 0) store_from_float(a.dpartner[n], c + i, p.dtype, by_weight);
+        store_from_float(a.dweight[n], c + i, w.dtype, per_sample ? sum[i] : sum[i] * vector_value(p, 0, c + i, n ? 1.f : 0.f, 1.f));
+      if (a.dpartner[n] != nullptr && !per_sample) store_from_float(a.dpartner[n], c + i, p.dtype, by_weight);
     }
   }
 }
@@ -309,6 +302,6 @@ extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGra
   t.by_sample = samples < t.units;
   const long long places = per_sample ? std::min(samples, t.units - 1) : 0;
   const long long sets = (places + 1) / 2 + (shared ? 1 : 0);
-  if (sets > 0) norm_sums_kernel<<<dim3((unsigned)sets, (n->cols + 127) / 128), 512, 0, stream>>>(t);
+  if (sets > 0) norm_sums_kernel<<<dim3((unsigned)sets, (n->cols + 127) / 128, 2), 512, 0, stream>>>(t);
   return (int)cudaGetLastError();
 }
