@@ -88,6 +88,7 @@ norm_sums_kernel(const NormSumArgs a) {
       by_partner[i] = per_sample ? 1.f : vector_value(p, 0, c + i, n ? 1.f : 0.f, 1.f);
     }
   }
+  cudaGridDependencySynchronize();              // from here on: what the backward kernel wrote
   float total[4] = {0.f, 0.f, 0.f, 0.f};
   const bool wide = a.cols % 4 == 0;
   for (long long u = first + turn; u < last; u += kAhead * stride) {
@@ -321,6 +322,17 @@ extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGra
   t.by_sample = samples < t.units;
   const long long places = per_sample ? std::min(samples, t.units - 1) : 0;
   const long long sets = (places + 1) / 2 + (shared ? 1 : 0);
-  if (sets > 0) norm_sums_kernel<<<dim3((unsigned)sets, (n->cols + 127) / 128, 2), 512, 0, stream>>>(t);
+  if (sets == 0) return 0;
+  // launched while the backward kernel's last blocks run: its blocks find their sums and read the vectors until then
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3((unsigned)sets, (n->cols + 127) / 128, 2);
+  config.blockDim = dim3(512);
+  config.stream = stream;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  cudaLaunchKernelEx(&config, norm_sums_kernel, t);
   return (int)cudaGetLastError();
 }

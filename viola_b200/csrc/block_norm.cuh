@@ -465,6 +465,7 @@ norm_backward_kernel(const NormArgs a) {
   __shared__ float buffer[2][3][32];
   using SX = Strip<TX, V, SHIFT>;
   using SY = Strip<TY, V, SHIFT>;
+  cudaTriggerProgrammaticLaunchCompletion();    // the kernel of the vectors' sums may start when there is room; it waits for this one
   const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
   const int groups = blockDim.x / threads;
   const TX* x = reinterpret_cast<const TX*>(a.x);
