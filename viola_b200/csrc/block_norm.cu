@@ -10,6 +10,7 @@
 #include <climits>
 
 #include "block_norm.cuh"
+#include "common/launch.cuh"
 
 namespace vb {
 
@@ -145,8 +146,12 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // every thread, so few threads with many values each take the fewest instructions: as many as four pieces a thread, as long
 // as not more lanes idle for it (128 x 256 x 1152, fp32 stream: 120 us with one piece a thread, 86 with three; 4 x 8192 x 4096
 // bf16: 254 and 202).  Backward: a piece takes three times the registers, and warps to hide latency count for more
-// (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four).  Shifted pieces
-// take more registers too: two a thread forward (4 x 4096 x 2047 bf16: 118 us with one, 103 with two, 133 with four).
+// (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four;
+// each with 8 us more for the vectors' sums
+// than now).  One norm at 80 registers, which makes six warps of a scheduler's four, won at 4 x 8192 x 2048 bf16 (149 to
+// 135 us) and lost where more row groups leave more sums (7175 x 1001 fp16 47 to 55, 128 x 256 x 1152 101 to 106): not kept.
+// Shifted pieces take more registers too: two a thread forward (4 x 4096 x 2047 bf16: 118 us with one, 103 with two, 133
+// with four).
 bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
   if (cols < 1 || cols > VB_NORM_MAX_COLS || (!shift && cols % kPiece)) return false;
   const int pieces = (cols + kPiece - 1) / kPiece;
@@ -324,15 +329,6 @@ extern "C" int vb_block_norm_backward(const VbBlockNorm* n, const VbBlockNormGra
   const long long sets = (places + 1) / 2 + (shared ? 1 : 0);
   if (sets == 0) return 0;
   // launched while the backward kernel's last blocks run: its blocks find their sums and read the vectors until then
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3((unsigned)sets, (n->cols + 127) / 128, 2);
-  config.blockDim = dim3(512);
-  config.stream = stream;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  cudaLaunchKernelEx(&config, norm_sums_kernel, t);
+  launch_early(norm_sums_kernel, dim3((unsigned)sets, (n->cols + 127) / 128, 2), 512, 0, stream, t);
   return (int)cudaGetLastError();
 }

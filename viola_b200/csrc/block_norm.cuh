@@ -446,8 +446,8 @@ norm_forward_kernel(const NormArgs a) {
 }
 
 // Bound by the latency of a row's load, reduction and store one after the other where few rows are in flight, by issued
-// instructions elsewhere: 4 x 8192 x 4096 bf16 354 us (70 % of the copy rate), 128 x 256 x 1152 with an fp32 stream 155 us
-// (67 %).
+// instructions elsewhere: 4 x 8192 x 4096 bf16 347 us (71 % of the copy rate), 128 x 256 x 1152 with an fp32 stream 146 us
+// (71 %).
 // With q = gate * weight * yh, t = dh * next_weight * (1 + next_scale), uh = u * ru, c = mean(t uh):
 //   d  = dout + ru (t - uh c)                  the gradient of u
 //   dx = alpha d,   dy = ry (d gate weight - yh m),   m = mean(d q)

@@ -11,6 +11,7 @@
 #include <climits>
 
 #include "api.h"
+#include "common/launch.cuh"
 #include "common/numerics.cuh"
 
 namespace vb {
@@ -168,13 +169,15 @@ template <int V> __device__ __forceinline__ void sort_keys(unsigned (&key)[V]) {
 // A lane sorts its (up to 16) keys; each choice then costs one maximum over the token's lanes and one step down the winner's
 // list in shared memory, and which expert a winning key belongs to is looked up for all choices at once.  More keys than
 // that are searched again for every choice.
-// Bound by the integer instructions it issues (131072 x 256, top 8, fp32: about 550 a token, 119 us for what 22 would
+// Bound by the integer instructions it issues (131072 x 256, top 8, fp32: about 550 a token, 113 us for what 22 would
 // read), many of them the same for a token whatever its experts: 16 lanes to a token put two tokens into each.  Keys
 // scanned again for every choice took 226 us, sorted together with their indices 140, ranked by pairs 120.
-// Four blocks an SM: 64 registers hold 16 keys a lane, and 32 warps hide the exchanges (119 us; 139 with 105 registers).
+// Four blocks an SM: 64 registers hold 16 keys a lane, and 32 warps hide the exchanges (119 us; 139 with 105 registers;
+// 113 once the finishing kernel had its loads under way together).
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256, V <= 16 ? 4 : 2)
 route_forward_kernel(const RouteArgs a) {
+  cudaTriggerProgrammaticLaunchCompletion();    // the finishing kernel may start when there is room; it waits for this one
   constexpr int kWarps = 8, kThreads = kWarps * 32;
   constexpr int kTokens = 32 / G;               // tokens a warp serves at a time
   constexpr bool kSorted = V > 1 && V <= 16;
@@ -389,24 +392,50 @@ route_forward_kernel(const RouteArgs a) {
 // Adds the blocks' sums in block order and derives the losses: one cluster, each block of which takes every eighth set of
 // 32 experts with 32 threads per expert; the first block adds the clusters' shares of the balance in order.
 constexpr int kFinishBlocks = 8;
+constexpr int kAhead = 8;                       // loads under way; they bound it
 __global__ void __cluster_dims__(kFinishBlocks, 1, 1) __launch_bounds__(1024)
 route_finish_kernel(const RouteArgs a, int blocks) {
   __shared__ float p_part[32][33];
   __shared__ int c_part[32][33];
   __shared__ float share[2];                    // this block's part of dot, and of choices as bits
+  __shared__ float z_part[32];
+  __shared__ int n_part[32];
   const int lane = threadIdx.x & 31, row = threadIdx.x >> 5;
   const long long pitch = 2 * a.experts + 2;
-  float dot = 0.f;
-  int choices = 0;
+  cudaGridDependencySynchronize();
+  float dot = 0.f, z = 0.f;
+  int choices = 0, n = 0;
+  if (blockIdx.x == 0) {
+    for (int b = threadIdx.x; b < blocks; b += 1024) {
+      z += a.partial[b * pitch + 2 * a.experts];
+      n += __float_as_int(a.partial[b * pitch + 2 * a.experts + 1]);
+    }
+    z = group_sum<32>(z);
+    n = __reduce_add_sync(kFull, n);
+    if (lane == 0) {
+      z_part[row] = z;
+      n_part[row] = n;
+    }
+    __syncthreads();
+  }
   for (int first = blockIdx.x * 32; first < a.experts; first += kFinishBlocks * 32) {
     const int e = first + lane;
     float p = 0.f;
     int c = 0;
-    if (e < a.experts) {
-#pragma unroll 4
-      for (int b = row; b < blocks; b += 32) {
-        p += a.partial[b * pitch + e];
-        c += __float_as_int(a.partial[b * pitch + a.experts + e]);
+    for (int b = row; b < blocks; b += 32 * kAhead) {
+      float ps[kAhead];
+      int cs[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const bool there = b + 32 * k < blocks && e < a.experts;
+        const float* at = a.partial + (b + 32 * k) * pitch + e;
+        ps[k] = there ? at[0] : 0.f;
+        cs[k] = there ? __float_as_int(at[a.experts]) : 0;
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        p += ps[k];
+        c += cs[k];
       }
     }
     p_part[row][lane] = p;
@@ -426,16 +455,9 @@ route_finish_kernel(const RouteArgs a, int blocks) {
     }
     __syncthreads();
   }
-  float z = 0.f;
-  int n = 0;
   if (blockIdx.x == 0 && row == 0) {
-#pragma unroll 4
-    for (int b = lane; b < blocks; b += 32) {
-      z += a.partial[b * pitch + 2 * a.experts];
-      n += __float_as_int(a.partial[b * pitch + 2 * a.experts + 1]);
-    }
-    z = group_sum<32>(z);
-    n = __reduce_add_sync(kFull, n);
+    z = group_sum<32>(z_part[lane]);
+    n = __reduce_add_sync(kFull, n_part[lane]);
   }
   if (threadIdx.x == 0) {
     share[0] = dot;
@@ -898,7 +920,7 @@ extern "C" int vb_route_forward(const void* logits, int dtype, int tokens, int e
   // at most 40 KB
   const size_t smem = ((size_t)(experts + 3) / 4 * 4 + lanes * per_lane) * 4 + std::max(lists, (size_t)8 * experts * sizeof(float));
   VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_forward_kernel<T, G, V><<<blocks, 256, smem, stream>>>(a))));
-  if (blocks > 1) route_finish_kernel<<<kFinishBlocks, 1024, 0, stream>>>(a, blocks);
+  if (blocks > 1) launch_early(route_finish_kernel, kFinishBlocks, 1024, 0, stream, a, blocks);
   return (int)cudaGetLastError();
 }
 
