@@ -863,3 +863,70 @@ def test_another_device_than_the_current_one():
     expected = whole_pass(*pass_leaves(11))
     for a, b in zip(expected, whole_pass(*leaves)):
         assert b.device.index == 1 and torch.equal(a.cpu(), b.cpu())
+
+
+# ------------------------------------------------------------------------------------------------------- forward mode
+def test_operators_refuse_tangents_before_anything_else():
+    """The operators read values alone: a tangent is refused, whether or not a gradient is asked for.  Needs no GPU."""
+    forward_ad = torch.autograd.forward_ad
+    library = ops._ops()
+    x, positions, offsets = torch.ones(4, 8), torch.zeros(4, 1, dtype=torch.int32), torch.tensor([0, 4], dtype=torch.int32)
+    vector, rows = torch.ones(8), torch.ones(4, 8)
+    calls = {
+        "route": lambda t: library.route(t, 2, None, None, True),
+        "dispatch": lambda t: library.expert_dispatch(t, positions, offsets),
+        "combine rows": lambda t: library.expert_combine(t, torch.ones(4, 1), positions, offsets),
+        "combine weights": lambda t: library.expert_combine(rows, t[:, :1], positions, offsets),
+        "norm x": lambda t: library.block_norm(t, None, None, None, None, None, 1.0, 1e-6, 0),
+        "norm y": lambda t: library.block_norm(x, t, None, None, None, None, 1.0, 1e-6, -1),
+        "norm weight": lambda t: library.block_norm(x, x, t[0], None, None, None, 1.0, 1e-6, -1),
+        "norm gate": lambda t: library.block_norm(x, x, vector, t[0], None, None, 1.0, 1e-6, -1),
+        "norm next weight": lambda t: library.block_norm(x, None, None, None, t[0], None, 1.0, 1e-6, 0),
+        "norm next scale": lambda t: library.block_norm(x, None, None, None, vector, t[0], 1.0, 1e-6, 0),
+    }
+    for name, call in calls.items():
+        for wants_grad in (False, True):
+            with forward_ad.dual_level():
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(forward_ad.make_dual(x.clone().requires_grad_(wants_grad), torch.ones_like(x)))
+                    pytest.fail(name)
+
+
+def test_tangents_reach_the_results_or_are_refused(device):
+    """A result never comes back without the tangent of its inputs: on the CPU it has one, on the GPU the call is refused.
+    The bias of the router moves the choice alone and has none to pass on."""
+    forward_ad = torch.autograd.forward_ad
+    x, vector = randn(0, 4, 8).to(device), randn(1, 8).to(device)
+    weights = torch.rand(4, 2, generator=torch.Generator().manual_seed(2)).to(device)
+    plan = nn.plan_experts(choices(4, 2, 3, dropped=0).to(device), 3)
+    for primal, call in ((x, lambda t: nn.route_tokens(t, 2).weights), (x, lambda t: nn.dispatch_tokens(t, plan)),
+                         (x.repeat(2, 1), lambda t: nn.combine_tokens(t, weights, plan)),
+                         (weights, lambda t: nn.combine_tokens(x.repeat(2, 1), t, plan)),
+                         (x, lambda t: nn.rms_norm_modulate(t)), (vector, lambda t: nn.rms_norm_modulate(x, t)),
+                         (vector, lambda t: nn.rms_norm_modulate(x, scale=t)), (x, lambda t: nn.rms_norm_residual(x, t)),
+                         (vector, lambda t: nn.rms_norm_residual(x, x, t)), (vector, lambda t: nn.rms_norm_residual(x, x, None, t))):
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(primal, torch.ones_like(primal))
+            if device == "cpu":
+                assert forward_ad.unpack_dual(call(dual)).tangent is not None
+            else:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(dual)
+    with forward_ad.dual_level():
+        biased = nn.route_tokens(x, 2, bias=forward_ad.make_dual(vector, torch.ones_like(vector)))
+        assert torch.equal(biased.indices, nn.route_tokens(x, 2, bias=vector).indices)
+
+
+@pytest.mark.gpu
+def test_tangents_of_gradients_are_refused():
+    forward_ad = torch.autograd.forward_ad
+    x = randn(0, 4, 8).cuda().requires_grad_(True)
+    weights = torch.rand(4, 2, generator=torch.Generator().manual_seed(2)).cuda()
+    plan = nn.plan_experts(choices(4, 2, 3, dropped=0).cuda(), 3)
+    rows = randn(1, 8, 8).cuda().requires_grad_(True)
+    for leaf, out in ((x, nn.route_tokens(x, 2).weights), (x, nn.dispatch_tokens(x, plan)),
+                      (rows, nn.combine_tokens(rows, weights, plan)), (x, nn.rms_norm_modulate(x))):
+        with forward_ad.dual_level():
+            grad = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(out, leaf, grad)

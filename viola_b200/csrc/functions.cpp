@@ -45,8 +45,15 @@ int narrow(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " out of range: ", v);
   return (int)v;
 }
-void once_only() {
+// A tangent would be lost without a word: the plain branches read the values alone, and so do the backward kernels.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... T> void no_tangents(const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(inputs) || ...), "viola_b200: these operators have no forward-mode derivatives on the GPU");
+}
+void once_only(const variable_list& grads) {
   TORCH_CHECK(!at::GradMode::is_enabled(), "viola_b200: the gradients of these operators cannot be differentiated again");
+  for (const Tensor& g : grads) no_tangents(g);
 }
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
@@ -131,7 +138,7 @@ struct Route : torch::autograd::Function<Route> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once_only();
+    once_only(grads);
     const Tensor &dbalance = grads[3], &dz = grads[4];
     if (!grads[0].defined() && !dbalance.defined() && !dz.defined()) return {none(), none(), none(), none(), none()};
     const variable_list saved = ctx->get_saved_variables();
@@ -151,6 +158,7 @@ struct Route : torch::autograd::Function<Route> {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> route(const Tensor& logits, int64_t top_k, const OptTensor& bias,
                                                          const OptTensor& mask, bool normalize) {
+  no_tangents(logits);         // one of the bias moves nothing
   if (at::GradMode::is_enabled() && wants_grad(logits)) {
     const variable_list out = Route::apply(logits, top_k, bias, mask, normalize);
     return {out[0], out[1], out[2], out[3], out[4]};
@@ -226,7 +234,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     return dispatch_forward(x, plan);
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once_only();
+    once_only(grads);
     const variable_list saved = ctx->get_saved_variables();
     const c10::cuda::CUDAGuard guard(saved[0].device());
     return {combine_forward(grads[0].contiguous(), none(), saved[0], ctx->saved_data["shape"].toIntVector()), none(), none()};
@@ -234,6 +242,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
 };
 
 Tensor expert_dispatch(const Tensor& x, const Tensor& positions, const Tensor& offsets) {
+  no_tangents(x);
   if (at::GradMode::is_enabled() && wants_grad(x)) return Dispatch::apply(x, positions, offsets);
   return dispatch_forward(x, check_plan(positions, offsets, x));
 }
@@ -258,7 +267,7 @@ struct Combine : torch::autograd::Function<Combine> {
     return combine_forward(r, w, positions, with_last(weights.sizes(), rows.size(1)));
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once_only();
+    once_only(grads);
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &rows = saved[0], &weights = saved[1], &positions = saved[2], &offsets = saved[3];
     const c10::cuda::CUDAGuard guard(rows.device());
@@ -276,6 +285,7 @@ struct Combine : torch::autograd::Function<Combine> {
 };
 
 Tensor expert_combine(const Tensor& rows, const Tensor& weights, const Tensor& positions, const Tensor& offsets) {
+  no_tangents(rows, weights);
   const Plan plan = check_combine(rows, weights, positions, offsets);
   if (at::GradMode::is_enabled() && (wants_grad(rows) || wants_grad(weights)))
     return Combine::apply(rows, weights, plan.positions, plan.offsets);
@@ -391,7 +401,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    once_only();
+    once_only(grads);
     variable_list result(9);
     const variable_list saved = ctx->get_saved_variables();
     Normed n;
@@ -436,6 +446,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
 std::vector<Tensor> block_norm(const Tensor& x, const OptTensor& y, const OptTensor& weight, const OptTensor& gate,
                                const OptTensor& next_weight, const OptTensor& next_scale, double residual_scale, double eps,
                                int64_t h_dtype) {
+  no_tangents(x, y, weight, gate, next_weight, next_scale);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(y) || wants_grad(weight) || wants_grad(gate) ||
                                      wants_grad(next_weight) || wants_grad(next_scale)))
     return BlockNorm::apply(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype);

@@ -11,7 +11,7 @@
 Nothing waits for the GPU: the row count is ``tokens * top_k`` whatever was chosen, and rows that no choice fills (tokens
 of a padded batch) are zero and lie behind the last expert's.  Results do not depend on the order in which the GPU runs
 its blocks.  CPU tensors take the same path through the PyTorch restatements.  On the GPU the gradients cannot be
-differentiated again.
+differentiated again, and inputs with forward-mode tangents are refused.
 """
 
 from __future__ import annotations

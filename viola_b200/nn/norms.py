@@ -10,7 +10,8 @@ follows it: the block's result ``y`` is normalised, gated and added to the scale
 Each call is one kernel forward and one (plus a small one for the gradients of the vectors) backward; nothing but two
 numbers per row is kept besides the inputs.  Vectors are [width] (shared by all rows) or [batch, width] with
 ``x`` [batch, ..., width] (one per sample, as an adaLN projection gives them).  CPU tensors take the same path through
-the PyTorch restatement.  On the GPU the gradients cannot be differentiated again.
+the PyTorch restatement.  On the GPU the gradients cannot be differentiated again, and inputs with forward-mode tangents are
+refused.
 """
 
 from __future__ import annotations
