@@ -930,3 +930,42 @@ def test_tangents_of_gradients_are_refused():
             grad = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 torch.autograd.grad(out, leaf, grad)
+
+
+# ----------------------------------------------------------------------------------- many rows to a group of the kernels
+# Row groups of the norms' kernels take equal shares of consecutive rows: at most 148 blocks times those an SM holds times 8,
+# 4, 2 or 1 rows at a time.  More rows than that put several to a group, and samples then begin and end inside one, cover it,
+# or reach over many.
+def check_many_rows(case, seed=0):
+    """As :func:`test_norm_values_and_gradients`, on the GPU; every sum has the terms that are its own."""
+    v, dout, dh = norm_inputs(case, seed)
+    batch, tokens, width = case[:3]
+    expected = oracle.block_norm(**v, residual_scale=case[10], next_norm=case[9], dout=dout, dh=dh)
+    leaves = {n: None if t is None else t.cuda().requires_grad_(True) for n, t in v.items()}
+    results = [(n, t, g) for n, t, g in zip(("out", "h"), call_norm(case, leaves), (dout, dh)) if t is not None]
+    torch.autograd.backward([t for _, t, _ in results], [g.cuda() for _, _, g in results])
+    for name, t, _ in results:
+        oracle.assert_matches(t, expected[name], width, name)
+    for name, leaf in leaves.items():
+        if leaf is not None:
+            rows = 0 if name in ("x", "y") else tokens if leaf.dim() == 2 else batch * tokens
+            oracle.assert_matches(leaf.grad, expected["d" + name], width + rows, "d" + name)
+
+
+MANY_NARROW_ROWS = [  # one warp a row, eight rows a block at a time
+    (6500, 3, 256, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (400, 50, 136, FP32, BF16, True, "sample", "sample", True, True, 0.8),
+    (23, 900, 40, FP16, FP16, True, "sample", "shared", True, True, 1.2),
+    (7001, 3, 131, FP32, FP32, True, "shared", "sample", True, True, 1.0),
+    (301, 67, 255, BF16, BF16, True, "sample", None, True, False, 0.5),
+    (900, 23, 64, FP32, FP16, True, None, "sample", False, True, 1.0),
+    (1, 20003, 72, FP32, BF16, True, "shared", "shared", True, True, 1.0),
+    (20003, 1, 48, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_NARROW_ROWS, ids=str)
+def test_norm_many_narrow_rows(case):
+    """With several samples the first use of a group's sums is behind no barrier where a row is one warp's."""
+    check_many_rows(case)

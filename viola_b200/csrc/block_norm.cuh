@@ -504,9 +504,11 @@ norm_backward_kernel(const NormArgs a) {
   float* gains = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)group * 2 * area;
   float* next_gains = gains + area;
   float* total = reinterpret_cast<float*>(ring + (size_t)groups * slots * a.slot_bytes) + (size_t)(groups + group) * 2 * area;
-  if (samples && a.totals_shared) {
-#pragma unroll 1
-    for (int k = 0; k < 2 * V * kPiece; ++k) total[k * threads + tid] = 0.f;
+  if (samples && a.totals_shared) {              // places that the thread itself adds to: no barrier
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < kPiece; ++i) total[own_place(j, i, tid, threads)] = total[area + own_place(j, i, tid, threads)] = 0.f;
   }
   const long long first_sample = samples ? first / a.tokens : 0;
   auto finish_norm = [&](int n, long long sample, const NormVector& weight, const NormVector& partner, float shift, void* grad,
