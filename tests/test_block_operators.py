@@ -969,3 +969,43 @@ MANY_NARROW_ROWS = [  # one warp a row, eight rows a block at a time
 def test_norm_many_narrow_rows(case):
     """With several samples the first use of a group's sums is behind no barrier where a row is one warp's."""
     check_many_rows(case)
+
+
+# ------------------------------------------------------------------------------------------------- the largest row counts
+@pytest.mark.parametrize("cols", [1, 40, 256, 1001, 1152, 16384])
+def test_norm_workspace_at_the_largest_row_counts(cols):
+    """The shares of a pass stop growing once every SM is full, up to the last row count that 31 bits hold.  Needs no GPU."""
+    import ctypes
+
+    ops.load()
+    workspace = ctypes.CDLL(str(ops._LIB_PATH)).vb_block_norm_workspace
+    workspace.restype = ctypes.c_longlong
+    for shared in (True, False):                                   # one sample, or two
+        full = workspace(1 << 20, cols, 1 << (20 if shared else 19))
+        for rows in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 8, 2 ** 31 - 600, 2 ** 30):
+            if shared or rows % 2 == 0:
+                assert full > 0 and workspace(rows, cols, rows if shared else rows // 2) == full, rows
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [2 ** 31 - 1, 2 ** 31 - 3000])
+def test_norm_at_the_largest_row_counts(rows):
+    """Every row of one value is written, forward and backward: x -> x / sqrt(x^2 + eps), dx = dh eps / (x^2 + eps)^(3/2)."""
+    values = torch.tensor([-2.0, -1.0, -0.5, 0.25, 0.5, 1.0, 3.0], device="cuda")
+    eps = 0.5                                                      # so that both results are far from zero
+    x = values.to(BF16).repeat((rows + 6) // 7)[:rows].view(rows, 1).requires_grad_(True)
+    h = nn.rms_norm_modulate(x, eps=eps)
+    wanted = (values.double() / (values.double() ** 2 + eps).sqrt())
+    slope = eps / (values.double() ** 2 + eps) ** 1.5
+    dx, = torch.autograd.grad(h, x, torch.ones_like(h))
+    for result, value in ((h.detach(), wanted), (dx, slope)):
+        # sums of one term, a root and four products in fp32, 16 steps of 2^-24 at most (the slope: of terms three times its
+        # size or less times a cancellation of 1 - uh^2 >= 1 / 19), and one rounding by 2^-8 of the value at most
+        low, high = (value - (2.0 ** -8 + 2.0 ** -14) * value.abs()).float(), (value + (2.0 ** -8 + 2.0 ** -14) * value.abs()).float()
+        low, high = torch.minimum(low, high), torch.maximum(low, high)
+        for first in range(0, rows, 7 << 25):                      # a multiple of the seven values at a time
+            part = result[first:first + (7 << 25), 0].float()
+            whole = part[:part.numel() // 7 * 7].view(-1, 7)
+            assert ((whole >= low) & (whole <= high)).all(), first
+            rest = part[whole.numel():]
+            assert ((rest >= low[:rest.numel()]) & (rest <= high[:rest.numel()])).all(), first

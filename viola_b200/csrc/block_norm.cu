@@ -185,6 +185,8 @@ struct NormPlan {
   int depth, slot_bytes, resident;
   size_t smem;
 };
+// blocks that give every row a group
+int row_blocks(int rows, const NormShape& s) { return (int)(((long long)rows + s.groups - 1) / s.groups); }
 int by_registers(const NormShape& s, int resident_threads) { return std::max(1, resident_threads / s.threads()); }
 NormPlan norm_plan(const NormShape& s, int piece_bytes, int areas, int resident_threads) {
   NormPlan p{0, 0, 1, 0};
@@ -227,7 +229,7 @@ bool totals_in_shared(const NormShape& s, int rows, int tokens) {
 bool backward_plan(int rows, int cols, int tokens, int bytes, bool shift, NormShape& s, NormPlan& p, int& blocks) {
   if (!norm_shape(cols, shift, true, s)) return false;
   p = norm_plan(s, bytes, totals_in_shared(s, rows, tokens) ? 4 : 2, kBackwardThreads);
-  blocks = std::min((rows + s.groups - 1) / s.groups, 148 * p.resident);
+  blocks = std::min(row_blocks(rows, s), 148 * p.resident);
   return true;
 }
 // sums of the shared vectors, and, with samples, what groups park
@@ -242,7 +244,7 @@ extern "C" long long vb_block_norm_workspace(int rows, int cols, int tokens) {
   if (rows <= 0 || cols <= 0 || tokens <= 0 || rows % tokens || cols > VB_NORM_MAX_COLS) return 0;
   NormShape s;
   if (!norm_shape(cols, true, true, s)) return 0;
-  const int blocks = std::min((rows + s.groups - 1) / s.groups, 148 * by_registers(s, kBackwardThreads));
+  const int blocks = std::min(row_blocks(rows, s), 148 * by_registers(s, kBackwardThreads));
   return backward_floats(s, blocks, rows, cols, tokens);
 }
 
@@ -265,7 +267,7 @@ extern "C" int vb_block_norm(const VbBlockNorm* n, cudaStream_t stream) {
   a.next_weight = to_vector(n->next_weight); a.next_scale = to_vector(n->next_scale);
   a.out = n->out; a.h = n->h; a.ry = n->ry; a.ru = n->ru;
   a.depth = p.depth; a.slot_bytes = p.slot_bytes;
-  const int blocks = (n->rows + s.groups - 1) / s.groups;
+  const int blocks = row_blocks(n->rows, s);
   if (launch_types(a, n->x_dtype, n->y_dtype, s, NormLaunch{false, post, pre, blocks, s.threads(), p.smem, stream}) == 0)
     return (int)cudaErrorInvalidValue;
   return (int)cudaGetLastError();

@@ -333,7 +333,7 @@ norm_forward_kernel(const NormArgs a) {
   using SY = Strip<TY, V, SHIFT>;
   const int threads = a.warps * 32, group = threadIdx.x / threads, tid = threadIdx.x - group * threads;
   const int groups = blockDim.x / threads, units = gridDim.x * groups;
-  const int per_unit = (a.rows + units - 1) / units;
+  const int per_unit = (int)(((unsigned)a.rows + units - 1u) / units);        // up to 2^31 - 1 rows
   const long long first = (long long)(blockIdx.x * groups + group) * per_unit;
   const long long last = min(first + per_unit, (long long)a.rows);
   const TX* x = reinterpret_cast<const TX*>(a.x);
