@@ -1009,3 +1009,19 @@ def test_norm_at_the_largest_row_counts(rows):
             assert ((whole >= low) & (whole <= high)).all(), first
             rest = part[whole.numel():]
             assert ((rest >= low[:rest.numel()]) & (rest <= high[:rest.numel()])).all(), first
+
+
+@pytest.mark.gpu
+def test_route_counts_choices_past_31_bits():
+    """2^31 choices and more: the balance loss divides by their number.  All tokens have the same logits (one row in memory), 16
+    of 17 experts are chosen: counts_e = tokens for the 16, balance = 17 / 16 * (1 - p of the other)."""
+    tokens, experts, top_k = 2 ** 27 + 5, 17, 16
+    row = torch.linspace(-1.0, 1.0, experts).to(FP16)
+    out = nn.route_tokens(row.cuda().expand(tokens, experts), top_k)
+    assert out.counts.tolist() == [0] + [tokens] * 16 and tokens * top_k > 2 ** 31
+    p = torch.softmax(row.double(), 0)
+    # a lane adds the p of tokens / (592 blocks * 16 tokens a pass) of them, each addition off by 2^-24 of the sum at most
+    off = (tokens / (592 * 16) + 700) * 2.0 ** -24
+    assert abs(float(out.balance_loss) / (17 / 16 * float(1 - p[0])) - 1) < off
+    assert abs(float(out.z_loss) / float(torch.logsumexp(row.double(), 0) ** 2) - 1) < off
+    assert int(out.indices[-1].sum()) == sum(range(1, 17)) and abs(float(out.weights[-1].sum()) - 1) < 1e-6
