@@ -1025,3 +1025,43 @@ def test_route_counts_choices_past_31_bits():
     assert abs(float(out.balance_loss) / (17 / 16 * float(1 - p[0])) - 1) < off
     assert abs(float(out.z_loss) / float(torch.logsumexp(row.double(), 0) ** 2) - 1) < off
     assert int(out.indices[-1].sum()) == sum(range(1, 17)) and abs(float(out.weights[-1].sum()) - 1) < 1e-6
+
+
+# ---------------------------------------------------------------------------------------------------- counted launches
+def test_launch_count_is_read_without_a_gpu():
+    before = ops.launch_count
+    ops._count(3)
+    assert ops.launch_count == before + 3
+    assert ops._ops().block_launches() >= 0 and not hasattr(ops, "launch_counts")
+
+
+@pytest.mark.gpu
+def test_launch_count_includes_the_block_operators():
+    def launched(call):
+        before = ops.launch_count
+        result = call()
+        return ops.launch_count - before, result
+
+    def logits(tokens):
+        return randn(0, tokens, 60).cuda().requires_grad_(True)
+
+    assert launched(lambda: nn.route_tokens(logits(1), 2))[0] == 1                # one block: no finishing kernel
+    count, routing = launched(lambda: nn.route_tokens(logits(5003), 4))
+    assert count == 2
+    assert launched(lambda: routing.z_loss.backward())[0] == 1
+    assert launched(lambda: nn.plan_experts(routing.indices[:9], 60))[0] == 1
+    count, plan = launched(lambda: nn.plan_experts(routing.indices, 60))
+    assert count == 2
+    x = randn(1, 5003, 64).cuda().requires_grad_(True)
+    count, rows = launched(lambda: nn.dispatch_tokens(x, plan))
+    assert count == 1 and launched(lambda: rows.backward(rows.detach(), retain_graph=True))[0] == 1
+    count, out = launched(lambda: nn.combine_tokens(rows.detach().requires_grad_(True), routing.weights.detach(), plan))
+    assert count == 1 and launched(lambda: out.backward(out.detach()))[0] == 1
+    count, h = launched(lambda: nn.rms_norm_modulate(x))
+    assert count == 1 and launched(lambda: h.backward(h.detach()))[0] == 1
+    weight = torch.ones(64, device="cuda", requires_grad=True)
+    count, h = launched(lambda: nn.rms_norm_modulate(x, weight))
+    assert count == 1 and launched(lambda: h.backward(h.detach()))[0] == 2       # and the kernel of the vectors' sums
+    assert launched(lambda: nn.route_tokens(torch.empty(0, 8, device="cuda"), 2))[0] == 1
+    none = nn.plan_experts(torch.empty(0, 2, dtype=torch.int32, device="cuda"), 3)
+    assert launched(lambda: nn.dispatch_tokens(torch.empty(0, 64, device="cuda"), none))[0] == 0

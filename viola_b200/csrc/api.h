@@ -214,6 +214,9 @@ int vb_expert_combine_backward(const void* dout, const void* rows, int dtype, in
                                const int* positions, const int* offsets, int experts, const void* weights,
                                int weight_dtype, void* drows, void* dweights, cudaStream_t stream);
 
+// kernels launched so far by the entries above and those of the next section
+long long vb_block_launches(void);
+
 // ---- RMS norms around a block (block_norm.cu) ----------------------------------------------------------
 //   out = residual_scale * x + gate * weight * y * ry,  ry = (mean(y^2) + eps)^-1/2     (with y)
 //   h   = out * ru * next_weight * (1 + next_scale)                                     (with h; out = x without y)

@@ -4,6 +4,7 @@
 #include <climits>
 
 #include "api.h"
+#include "common/launch.cuh"
 #include "common/numerics.cuh"
 
 namespace vb {
@@ -747,6 +748,7 @@ int launch_kernel(const NormArgs& a, const NormLaunch& l) {
   if (l.smem > 48 * 1024 - 1024) allow_shared<Kernel>();
   const int room = 148 * resident_blocks<Kernel>(l.threads, l.smem), blocks = l.blocks < room ? l.blocks : room;
   Kernel<<<blocks, l.threads, l.smem, l.stream>>>(a);
+  count_launch();
   return blocks;
 }
 

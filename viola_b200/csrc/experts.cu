@@ -866,6 +866,8 @@ combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, 
 
 using namespace vb;
 
+extern "C" long long vb_block_launches(void) { return launches.load(std::memory_order_relaxed); }
+
 static bool aligned_to(const void* p, long long bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 // lanes per token (G) and experts per lane (V)
@@ -931,6 +933,7 @@ extern "C" int vb_route_forward(const void* logits, int dtype, int tokens, int e
   // at most 40 KB
   const size_t smem = ((size_t)(experts + 3) / 4 * 4 + lanes * per_lane) * 4 + std::max(lists, (size_t)8 * experts * sizeof(float));
   VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_forward_kernel<T, G, V><<<blocks, 256, smem, stream>>>(a))));
+  count_launch();
   if (blocks > 1) launch_early(route_finish_kernel, kFinishBlocks, 1024, 0, stream, a, blocks);
   return (int)cudaGetLastError();
 }
@@ -948,6 +951,7 @@ extern "C" int vb_route_backward(const void* logits, int dtype, int tokens, int 
   const long long per_pass = 8LL * (32 / lanes);
   const int blocks = (int)std::min<long long>((tokens + per_pass - 1) / per_pass, 148LL * 8);
   VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_backward_kernel<T, G, V><<<blocks, 256, 0, stream>>>(a))));
+  count_launch();
   return (int)cudaGetLastError();
 }
 
@@ -970,7 +974,10 @@ extern "C" int vb_expert_plan(const void* indices, int is_long, int n, int exper
   const int chunk = plan_chunk(n), blocks = n <= chunk ? 1 : (int)(((long long)n + chunk - 1) / chunk);
   int columns = 32;
   while (columns < experts) columns *= 2;
-  if (blocks > 1) plan_count_kernel<<<blocks, 512, experts * sizeof(int), stream>>>(indices, is_long, n, experts, chunk, workspace);
+  if (blocks > 1) {
+    plan_count_kernel<<<blocks, 512, experts * sizeof(int), stream>>>(indices, is_long, n, experts, chunk, workspace);
+    count_launch();
+  }
   const int* histogram = blocks > 1 ? workspace : nullptr;
   if (experts <= 512)
     plan_place_kernel<16><<<blocks, 512, 18 * (size_t)experts * sizeof(int), stream>>>(indices, is_long, n, experts, columns, chunk,
@@ -978,6 +985,7 @@ extern "C" int vb_expert_plan(const void* indices, int is_long, int n, int exper
   else                                           // 8 warps' counts of more experts fit 48 KB
     plan_place_kernel<8><<<blocks, 256, 10 * (size_t)experts * sizeof(int), stream>>>(indices, is_long, n, experts, columns, chunk,
                                                                                      histogram, offsets, positions);
+  count_launch();
   return (int)cudaGetLastError();
 }
 
@@ -1016,6 +1024,7 @@ extern "C" int vb_expert_dispatch(const void* x, long long x_stride_bytes, long 
   else if (unit == 8) launch(uint2{});
   else if (unit == 4) launch(uint32_t{});
   else launch(uint16_t{});
+  count_launch();
   return (int)cudaGetLastError();
 }
 
@@ -1044,6 +1053,7 @@ extern "C" int vb_expert_combine(const void* rows, int dtype, int width, int tok
     else if (per_lane == 5) launch(combine_kernel<T, 1, 5>);
     else launch(combine_kernel<T, 1, 8>);
   });
+  count_launch();
   return (int)cudaGetLastError();
 }
 
@@ -1072,5 +1082,6 @@ extern "C" int vb_expert_combine_backward(const void* dout, const void* rows, in
     else if (per_lane <= 2) launch(combine_backward_kernel<T, 1, 2>);
     else launch(combine_backward_kernel<T, 1, 4>);
   });
+  count_launch();
   return (int)cudaGetLastError();
 }

@@ -12,7 +12,6 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 #include <algorithm>
-#include <atomic>
 #include <cmath>
 #include <limits>
 #include <optional>
@@ -29,17 +28,14 @@ using torch::autograd::variable_list;
 
 constexpr int64_t kMaxExperts = 1024, kMaxTopK = 32, kMaxWidth = 1 << 22;
 
-std::atomic<int64_t> launches{0};     // kernels launched from here (bench bookkeeping)
-
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 int dtype_code(at::ScalarType t) {
   TORCH_CHECK_TYPE(t == at::kFloat || t == at::kBFloat16 || t == at::kHalf, "expected float32, bfloat16 or float16, got ", t);
   return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : 2;
 }
-void check(int rc, const char* what, int kernels) {
+void check(int rc, const char* what) {
   TORCH_CHECK(rc == 0, "viola_b200::", what, " failed: ", cudaGetErrorString((cudaError_t)rc), " (", rc, ")");
-  launches.fetch_add(kernels, std::memory_order_relaxed);
 }
 int narrow(int64_t v, const char* name) {
   TORCH_CHECK_VALUE(v >= 0 && v <= INT32_MAX, name, " out of range: ", v);
@@ -120,7 +116,7 @@ Routed route_forward(const Tensor& logits, int64_t top_k, const OptTensor& bias,
                          (const uint8_t*)ptr(live), (int)top_k, normalize, r.weights.data_ptr<float>(),
                          r.indices.data_ptr<int>(), r.counts.data_ptr<int>(), r.balance.data_ptr<float>(),
                          r.z.data_ptr<float>(), save ? r.inverse.data_ptr<float>() : work + need, work, need, stream()),
-        "route_forward", 1);
+        "route_forward");
   return r;
 }
 
@@ -151,7 +147,7 @@ struct Route : torch::autograd::Function<Route> {
                             saved[1].data_ptr<float>(), indices.data_ptr<int>(), saved[3].data_ptr<int>(),
                             saved[4].data_ptr<float>(), (const float*)ptr(dweights), (const float*)ptr(dbalance),
                             (const float*)ptr(dz), dlogits.data_ptr(), stream()),
-          "route_backward", 1);
+          "route_backward");
     return {dlogits.view(ctx->saved_data["shape"].toIntVector()), none(), none(), none(), none()};
   }
 };
@@ -184,7 +180,7 @@ std::tuple<Tensor, Tensor> expert_plan(const Tensor& indices, int64_t experts) {
   if (need) workspace = at::empty({need}, i32);
   check(vb_expert_plan(ptr(flat), flat.scalar_type() == at::kLong, n, e, offsets.data_ptr<int>(), positions.data_ptr<int>(),
                        (int*)ptr(workspace), need, stream()),
-        "expert_plan", need ? 2 : 1);
+        "expert_plan");
   return {offsets, positions};
 }
 
@@ -207,7 +203,7 @@ Tensor combine_forward(const Tensor& rows, const Tensor& weights, const Tensor& 
   check(vb_expert_combine(ptr(rows), dtype_code(rows.scalar_type()), narrow(rows.size(1), "width"), (int)positions.size(0),
                           (int)positions.size(1), positions.data_ptr<int>(), ptr(weights),
                           weights.defined() ? dtype_code(weights.scalar_type()) : 0, ptr(out), stream()),
-        "expert_combine", 1);
+        "expert_combine");
   return out;
 }
 
@@ -222,7 +218,7 @@ Tensor dispatch_forward(const Tensor& x, const Plan& plan) {
   Tensor rows = at::empty({positions.numel(), width}, x.options());
   check(vb_expert_dispatch(ptr(flat), flat.stride(0) * flat.element_size(), width * flat.element_size(), plan.tokens, plan.top_k,
                            positions.data_ptr<int>(), offsets.data_ptr<int>(), plan.experts, ptr(rows), stream()),
-        "expert_dispatch", 1);
+        "expert_dispatch");
   return rows;
 }
 
@@ -279,7 +275,7 @@ struct Combine : torch::autograd::Function<Combine> {
                                      (int)positions.size(0), (int)positions.size(1), positions.data_ptr<int>(),
                                      offsets.data_ptr<int>(), (int)offsets.numel() - 1, ptr(weights),
                                      dtype_code(weights.scalar_type()), ptr(drows), ptr(dweights), stream()),
-          "expert_combine_backward", 1);
+          "expert_combine_backward");
     return {drows, dweights, none(), none()};
   }
 };
@@ -376,7 +372,7 @@ Normed norm_forward(const Tensor& x, const OptTensor& y, const OptTensor& weight
   n.args = norm_args(n, rows, cols, n.tokens, residual_scale, eps, y_dtype);
   n.args.out = ptr(n.out);
   n.args.h = ptr(n.h);
-  check(vb_block_norm(&n.args, stream()), "block_norm", 1);
+  check(vb_block_norm(&n.args, stream()), "block_norm");
   return n;
 }
 
@@ -438,7 +434,7 @@ struct BlockNorm : torch::autograd::Function<BlockNorm> {
       workspace = at::empty({(int64_t)g.workspace_floats}, n.x.options().dtype(at::kFloat));
       g.workspace = workspace.data_ptr<float>();
     }
-    check(vb_block_norm_backward(&a, &g, stream()), "block_norm_backward", sums ? 2 : 1);
+    check(vb_block_norm_backward(&a, &g, stream()), "block_norm_backward");
     return result;
   }
 };
@@ -453,7 +449,7 @@ std::vector<Tensor> block_norm(const Tensor& x, const OptTensor& y, const OptTen
   return norm_results(norm_forward(x, y, weight, gate, next_weight, next_scale, residual_scale, eps, h_dtype, false));
 }
 
-int64_t block_launches() { return launches.load(std::memory_order_relaxed); }
+int64_t block_launches() { return vb_block_launches(); }
 
 }  // namespace
 

@@ -32,7 +32,14 @@ _ACT = {"silu": 0, "gelu": 1, "relu": 2}
 EPI_LINEAR, EPI_AXPBY, EPI_GATED_FWD, EPI_GATED_BWD, EPI_ACT_BWD = 0, 1, 2, 3, 4
 _NO_GROUP = (0, 0, 0, 0, 0, 0, 0)
 
-launch_count = 0  # number of library kernels launched through this layer (bench bookkeeping)
+_launches = 0    # library kernels launched from Python, see ``launch_count``
+
+
+def __getattr__(name):
+    # ``launch_count``: library kernels launched so far (bench bookkeeping), those of csrc/functions.cpp among them
+    if name == "launch_count":
+        return _launches + (_block_op("block_launches")() if _loaded else 0)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def load(build_if_missing: bool = True):
@@ -61,8 +68,8 @@ def _ops():
 
 
 def _count(n=1):
-    global launch_count
-    launch_count += n
+    global _launches
+    _launches += n
 
 
 # ------------------------------------------------------------------------------ workspaces
@@ -891,7 +898,7 @@ def gate_residual_backward(dout, gate, y, tokens, sums_dtype=torch.float32):
 
 # ------------------------------------------------------------------------------ expert routing
 # These operators and the norms below allocate their results and record their gradients in C++ (csrc/functions.cpp);
-# :func:`block_launches` counts the kernels launched there.  On the CPU autograd differentiates the restatements.
+# ``launch_count`` includes the kernels launched there.  On the CPU autograd differentiates the restatements.
 MAX_EXPERTS, MAX_TOP_K, MAX_DISPATCH_WIDTH = 1024, 32, 1 << 22
 _block_ops = {}
 
@@ -901,11 +908,6 @@ def _block_op(name):
     if op is None:
         op = _block_ops[name] = getattr(_ops(), name).default
     return op
-
-
-def block_launches():
-    """Kernels launched so far by the operators that record their own gradients."""
-    return _block_op("block_launches")()
 
 
 def route(logits, top_k, *, bias=None, mask=None, normalize=True):
