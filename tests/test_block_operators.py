@@ -1065,3 +1065,21 @@ def test_launch_count_includes_the_block_operators():
     assert launched(lambda: nn.route_tokens(torch.empty(0, 8, device="cuda"), 2))[0] == 1
     none = nn.plan_experts(torch.empty(0, 2, dtype=torch.int32, device="cuda"), 3)
     assert launched(lambda: nn.dispatch_tokens(torch.empty(0, 64, device="cuda"), none))[0] == 0
+
+
+@pytest.mark.parametrize("columns, out_dtype", [(64, FP32), (200, BF16), (68, BF16), (1152, BF16)])
+def test_expert_gemm_clears_many_rows_behind_the_last_experts(columns, out_dtype, device):
+    """More rows than the clearing warps take at a time, rows on and off 16 bytes, and nothing to clear."""
+    rows, experts = 5003, 2
+    q, _ = ops.quantize(randn(1, rows, 128).to(device), torch.ones(1, device=device))
+    w, _ = ops.quantize(randn(2, experts * columns, 128).to(device), torch.ones(1, device=device))
+    scale = torch.ones(1, device=device)
+    results = []
+    for used in (0, 17, 2600, rows):
+        offsets = torch.tensor([0, used // 2, used], dtype=torch.int32, device=device)
+        dirt = torch.full((rows, columns), math.nan, dtype=out_dtype, device=device)      # what the allocator may hand out again
+        del dirt
+        y = ops.expert_gemm(q, w.view(experts, columns, 128), offsets, scale, scale, out_dtype=out_dtype)
+        assert y[used:].eq(0).all() and y[:used].isfinite().all() and y[:used].ne(0).any(1).all()
+        results.append(y)
+    assert torch.equal(results[2][:8], results[1][:8]) and torch.equal(results[2][2592:2600], results[3][2592:2600])
