@@ -175,3 +175,58 @@ def block_norm(x, y, weight=None, gate=None, next_weight=None, next_scale=None, 
             d, ds = residual_scale * d, abs(residual_scale) * ds
         result["dx"] = (d, ds)
     return result
+
+
+def route_batch(logits, top_k, *, bias=None, mask=None, normalize=True, dweights=None, dbalance=0.0, dz=0.0):
+    """:func:`route` for many tokens at once: the same definitions and term sizes over whole tensors."""
+    tokens, experts = logits.shape
+    live = torch.ones(tokens, dtype=torch.bool) if mask is None else mask.cpu()
+    l32 = torch.where(live[:, None], logits.detach().cpu().float(), -math.inf)
+    key = l32 if bias is None else l32 + bias.detach().cpu().float()
+    order = torch.argsort(-key, dim=1, stable=True)[:, :top_k]
+    open_ = key.gather(1, order) != -math.inf
+    live = live & open_[:, 0]
+    l = torch.where(live[:, None], l32, 0.0).double()
+    picked = torch.zeros(tokens, experts, dtype=torch.bool).scatter_(1, order, open_) & live[:, None]
+    p = torch.softmax(l, 1) * live[:, None]
+    lse = torch.logsumexp(l, 1) * live
+    if normalize:
+        w = torch.softmax(torch.where(picked, l, -math.inf), 1).nan_to_num(0) * picked
+    else:
+        w = p * picked
+    counts = picked.sum(0)
+    n, choices = max(1, int(live.sum())), max(1, int(counts.sum()))
+    share = counts.double() / choices
+    balance, z = experts * (share * p.sum(0)).sum() / n, (lse * lse).sum() / n
+    weights, spread = w.gather(1, order) * open_, 1 + l.nan_to_num(0, 0, 0).abs().amax(1, keepdim=True)
+    result = dict(weights=(weights, weights * spread), indices=torch.where(open_ & live[:, None], order, -1).to(torch.int32),
+                  counts=counts.to(torch.int32), balance=(balance, balance.abs() * 4), z=(z, z.abs() * 4 + 1e-30))
+    if dweights is not None or dbalance or dz:
+        grad, size = torch.zeros_like(p), torch.zeros_like(p)
+        if dweights is not None:
+            g = torch.zeros_like(p).scatter_(1, order, dweights.cpu().double() * open_) * live[:, None]
+            dot, dot_size = (w * g).sum(1, keepdim=True), (w * g).abs().sum(1, keepdim=True)
+            over = w if normalize else p
+            grad += w * g - over * dot
+            size += (w * g).abs() + over * dot_size
+        mean = (p * share).sum(1, keepdim=True)
+        grad += dbalance * experts / n * p * (share - mean) + dz * 2 / n * lse[:, None] * p
+        size += abs(dbalance) * experts / n * p * (share + mean) + abs(dz) * 2 / n * lse[:, None].abs() * p
+        size *= 2 + torch.where(l.isfinite(), l, 0.0).abs().amax(1, keepdim=True)
+        result["dlogits"] = (grad, size)
+    return result
+
+
+def combine_batch(rows, weights, positions, dout=None):
+    """:func:`combine` for many tokens at once."""
+    rows, weights, at = rows.detach().cpu().double(), weights.detach().cpu().double().view(positions.shape), positions.cpu().long()
+    there = at >= 0
+    factor, taken = weights * there, rows[at.clamp_min(0)] * there[..., None]
+    terms = factor[..., None] * taken
+    result = dict(out=(terms.sum(1), terms.abs().sum(1)))
+    if dout is not None:
+        g = dout.detach().cpu().double()[:, None]
+        drows = torch.zeros_like(rows)
+        drows[at[there]] = (factor[..., None] * g)[there]
+        result.update(drows=(drows, drows.abs()), dweights=((g * taken).sum(2), (g * taken).abs().sum(2)))
+    return result

@@ -1083,3 +1083,142 @@ def test_expert_gemm_clears_many_rows_behind_the_last_experts(columns, out_dtype
         assert y[used:].eq(0).all() and y[:used].isfinite().all() and y[:used].ne(0).any(1).all()
         results.append(y)
     assert torch.equal(results[2][:8], results[1][:8]) and torch.equal(results[2][2592:2600], results[3][2592:2600])
+
+
+# --------------------------------------------------------------------------- shares of more than one row, token or block
+MANY_ROWS = [  # batch, tokens, width, stream, branch, weights, gate, scale, post, pre, residual; 8 to 1 rows a block at a time
+    (1500, 4, 264, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (1201, 5, 511, FP32, BF16, True, "sample", "sample", True, True, 0.7),
+    (700, 5, 520, FP16, FP16, True, "shared", "sample", True, True, 1.0),
+    (9, 401, 771, FP32, FP32, True, "sample", "sample", True, True, 1.1),
+    (1000, 3, 1152, FP32, BF16, True, "sample", "sample", True, True, 1.0),
+    (12, 251, 1152, BF16, BF16, True, "sample", "sample", True, True, 0.5),
+    (2000, 1, 1152, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (1, 4001, 1152, FP32, BF16, True, "shared", "shared", True, True, 1.0),
+    (64, 51, 1152, FP32, FP16, True, None, "sample", False, True, 1.0),
+    (64, 51, 1152, FP32, BF16, True, "sample", None, True, False, 1.0),
+    (7, 1025, 1001, FP16, FP16, True, "sample", None, True, False, 0.5),
+    (150, 5, 2056, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (3, 251, 2049, FP32, BF16, False, "sample", "shared", True, True, 1.0),
+    (60, 13, 4104, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (5, 125, 4099, FP16, FP16, True, "sample", "sample", True, True, 1.0),
+    (45, 11, 8200, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+    (2, 211, 8201, FP32, BF16, True, "shared", "sample", True, True, 1.0),
+    (7, 61, 16384, BF16, BF16, True, "sample", "sample", True, True, 1.0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_ROWS, ids=str)
+def test_norm_many_rows(case):
+    check_many_rows(case)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [1, 3])
+@pytest.mark.parametrize("case", [MANY_ROWS[0], MANY_ROWS[4], MANY_NARROW_ROWS[1]], ids=str)
+def test_norm_many_rows_off_their_boundary(case, offset):
+    """Aligned widths behind pointers that are not: every row is shifted by the same bytes."""
+    v, dout, dh = norm_inputs(case, 5)
+    batch, tokens, width = case[:3]
+    expected = oracle.block_norm(**v, residual_scale=case[10], dout=dout, dh=dh)
+    moved = {n: torch.cat([t.new_zeros(offset), t.reshape(-1)]).cuda()[offset:].view(t.shape) for n, t in v.items() if n in ("x", "y")}
+    leaves = {n: moved.get(n, t.cuda()).requires_grad_(True) for n, t in v.items()}
+    out, h = call_norm(case, leaves)
+    torch.autograd.backward([out, h], [dout.cuda(), dh.cuda()])
+    for name, t in (("out", out), ("h", h)):
+        oracle.assert_matches(t, expected[name], width, name)
+    for name, leaf in leaves.items():
+        rows = 0 if name in ("x", "y") else tokens if leaf.dim() == 2 else batch * tokens
+        oracle.assert_matches(leaf.grad, expected["d" + name], width + rows, "d" + name)
+
+
+@pytest.mark.parametrize("case", ROUTES, ids=str)
+def test_batched_route_oracle(case):
+    """The two oracles of the router agree: only then does the one for many tokens stand for the other."""
+    logits, bias, mask, (dw, db, dz) = route_inputs(case, 1)
+    one = oracle.route(logits, case[2], bias=bias, mask=mask, normalize=case[6], dweights=dw, dbalance=db, dz=dz)
+    many = oracle.route_batch(logits, case[2], bias=bias, mask=mask, normalize=case[6], dweights=dw, dbalance=db, dz=dz)
+    assert torch.equal(one["indices"], many["indices"]) and torch.equal(one["counts"], many["counts"])
+    for name in ("weights", "balance", "z", "dlogits"):
+        torch.testing.assert_close(many[name][0], one[name][0], rtol=1e-11, atol=1e-14)
+
+
+MANY_TOKENS = [  # tokens, experts, top_k, ... as above: more than 592 blocks take at a time, or than 256 blocks' sums a finishing thread
+    (40003, 4, 2, FP32, False, 0.1, True, 3),
+    (20011, 8, 2, BF16, True, 0, False, 0),
+    (12011, 60, 4, FP16, True, 0.2, False, 0),
+    (9973, 256, 8, FP32, True, 0, True, 0),
+    (10007, 256, 3, BF16, False, 0.3, True, 6),
+    (5003, 129, 20, FP16, True, 0.1, True, 0),
+    (4999, 512, 8, FP32, False, 0, False, 0),
+    (4801, 1024, 8, BF16, True, 0.1, True, 0),
+    (2500, 1000, 32, FP32, True, 0, True, 0),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_TOKENS, ids=str)
+def test_route_many_tokens(case):
+    tokens, experts, top_k, _, _, _, normalize, _ = case
+    logits, bias, mask, (dw, db, dz) = route_inputs(case)
+    expected = oracle.route_batch(logits, top_k, bias=bias, mask=mask, normalize=normalize, dweights=dw, dbalance=db, dz=dz)
+    leaf = logits.cuda().requires_grad_(True)
+    out = nn.route_tokens(leaf, top_k, bias=None if bias is None else bias.cuda(), mask=None if mask is None else mask.cuda(),
+                          normalize=normalize)
+    assert torch.equal(out.indices.cpu(), expected["indices"]) and torch.equal(out.counts.cpu(), expected["counts"])
+    oracle.assert_matches(out.weights, expected["weights"], experts, "weights")
+    # the losses' sums go through a lane's tokens (at most tokens / 4736), 5 exchanges, 8 warps, 19 of 592 blocks and 32 rows
+    depth = experts + tokens // 4736 + 1 + 5 + 8 + 19 + 32
+    oracle.assert_matches(out.balance_loss, expected["balance"], depth, "balance")
+    oracle.assert_matches(out.z_loss, expected["z"], depth, "z")
+    (out.weights * dw.cuda()).sum().add(db * out.balance_loss).add(dz * out.z_loss).backward()
+    oracle.assert_matches(leaf.grad, expected["dlogits"], experts, "dlogits")
+
+
+MANY_EXCHANGES = [  # tokens, top_k, experts, width, dtype: 2, 5 and 8 packs a lane, of 16 bytes and of one value, 1 to 8 warps a row
+    (2400, 2, 16, 1152, BF16), (2500, 2, 8, 2048, BF16), (2400, 3, 9, 771, FP16), (3001, 2, 5, 145, FP32),
+    (2400, 2, 8, 1000, FP32), (5001, 4, 7, 64, FP16), (2369, 1, 3, 4104, BF16), (2400, 2, 4, 2047, BF16),
+]
+
+
+@pytest.mark.parametrize("case", EXCHANGES, ids=str)
+def test_batched_combine_oracle(case):
+    tokens, top_k, experts, width, dtype = case
+    _, positions = oracle.plan(choices(tokens, top_k, experts, seed=2), experts)
+    rows, weights, dout = randn(3, tokens * top_k, width, dtype=dtype), randn(4, tokens, top_k), randn(5, tokens, width, dtype=dtype)
+    one, many = oracle.combine(rows, weights, positions, dout), oracle.combine_batch(rows, weights, positions, dout)
+    for name in one:
+        torch.testing.assert_close(many[name], one[name], rtol=1e-12, atol=1e-14)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", MANY_EXCHANGES, ids=str)
+@pytest.mark.parametrize("weight_dtype", [FP32, FP16])
+def test_exchange_of_many_tokens(case, weight_dtype):
+    tokens, top_k, experts, width, dtype = case
+    indices = choices(tokens, top_k, experts, seed=2)
+    plan = nn.plan_experts(indices.cuda(), experts)
+    positions, last = plan.positions.cpu(), int(plan.offsets[-1])
+    placed = positions >= 0
+    assert int(placed.sum()) == last and torch.equal(positions[placed].long().sort().values, torch.arange(last))
+    x = randn(0, tokens, width, dtype=dtype)
+    leaf = x.cuda().requires_grad_(True)
+    sent = nn.dispatch_tokens(leaf, plan)
+    expected = torch.zeros(tokens * top_k, width, dtype=dtype)
+    expected[positions[placed].long()] = x[placed.nonzero(as_tuple=True)[0]]
+    assert torch.equal(sent.detach().cpu(), expected)
+    grad = randn(1, tokens * top_k, width, dtype=dtype)
+    sent.backward(grad.cuda())
+    oracle.assert_matches(leaf.grad, oracle.combine_batch(grad, torch.ones(tokens, top_k), positions)["out"], top_k, "dx")
+    rows = randn(3, tokens * top_k, width, dtype=dtype)
+    rows[last:] = math.nan
+    weights = torch.rand(tokens, top_k, generator=torch.Generator().manual_seed(4)).to(weight_dtype)
+    dout = randn(5, tokens, width, dtype=dtype)
+    expected = oracle.combine_batch(rows.nan_to_num(0), weights, positions, dout)
+    leaf, wleaf = rows.cuda().requires_grad_(True), weights.cuda().requires_grad_(True)
+    out = nn.combine_tokens(leaf, wleaf, plan)
+    oracle.assert_matches(out, expected["out"], top_k, "out")
+    out.backward(dout.cuda())
+    oracle.assert_matches(leaf.grad, expected["drows"], 1, "drows")
+    oracle.assert_matches(wleaf.grad, expected["dweights"], width, "dweights")
