@@ -202,7 +202,7 @@ long long vb_expert_plan_workspace(int n, int experts);
 int vb_expert_plan(const void* indices, int is_long, int n, int experts, int* offsets, int* positions, int* workspace,
                    long long workspace_ints, cudaStream_t stream);
 // rows[positions[t, j]] = x[t] byte for byte (rows of an even number of bytes); rows from offsets[experts] on are zeroed.
-// Positions outside [0, tokens * top_k) are skipped, here and below.
+// Positions outside [0, tokens * top_k) are skipped, here and below; a row below offsets[experts] that none names is not written.
 int vb_expert_dispatch(const void* x, long long x_stride_bytes, long long row_bytes, int tokens, int top_k,
                        const int* positions, const int* offsets, int experts, void* rows, cudaStream_t stream);
 // out[t] = sum_j weights[t, j] * rows[positions[t, j]] (weights null: 1), accumulated in fp32

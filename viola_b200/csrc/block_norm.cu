@@ -149,9 +149,10 @@ bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // (the same: 154 us with one piece, 171 with two, 237 with three; 356 with one, 380 with two, 530 with four;
 // each with 8 us more for the vectors' sums
 // than now).  One norm at 80 registers, which makes six warps of a scheduler's four, won at 4 x 8192 x 2048 bf16 (149 to
-// 135 us) and lost where more row groups leave more sums (7175 x 1001 fp16 47 to 55, 128 x 256 x 1152 101 to 106): not kept.
+// 135 us; the norm behind a block takes 144 now, 57 % of the copy rate, the one in front of it 113, 55 %) and lost where more row
+// groups leave more sums (7175 x 1001 fp16 47 to 55, 128 x 256 x 1152 101 to 106): not kept.
 // Shifted pieces take more registers too: two a thread forward (4 x 4096 x 2047 bf16: 118 us with one, 103 with two, 133
-// with four).
+// with four; 100 now).
 bool norm_shape(int cols, bool shift, bool backward, NormShape& s) {
   if (cols < 1 || cols > VB_NORM_MAX_COLS || (!shift && cols % kPiece)) return false;
   const int pieces = (cols + kPiece - 1) / kPiece;

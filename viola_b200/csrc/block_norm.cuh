@@ -447,8 +447,10 @@ norm_forward_kernel(const NormArgs a) {
 }
 
 // Bound by the latency of a row's load, reduction and store one after the other where few rows are in flight, by issued
-// instructions elsewhere: 4 x 8192 x 4096 bf16 347 us (71 % of the copy rate), 128 x 256 x 1152 with an fp32 stream 146 us
-// (71 %).
+// instructions elsewhere: 4 x 8192 x 4096 bf16 349 us (70 % of the copy rate), 128 x 256 x 1152 with an fp32 stream 146 us
+// (71 %).  Wider rows spill, as d, yh, uh and the two column sums wait for the row's sums in registers: two pieces a thread (more
+// than 4096 columns) 80 to 128 bytes, four (more than 8192) 464 to 736, shifted 96 to 272 and 1320 to 1832.  2 x 4096 x 8192 bf16
+// takes 181 us (68 %), 2 x 2048 x 16384 351 (35 %).
 // With q = gate * weight * yh, t = dh * next_weight * (1 + next_scale), uh = u * ru, c = mean(t uh):
 //   d  = dout + ru (t - uh c)                  the gradient of u
 //   dx = alpha d,   dy = ry (d gate weight - yh m),   m = mean(d q)

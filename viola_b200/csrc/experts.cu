@@ -109,7 +109,9 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 
 // e[i] = exp(l[i] - top) with top the row's maximum; returns their sum.  The hardware's base-2 exponential is off by about
-// 2^-22 of its value and its argument by 2^-24 |l - top|, a few steps of fp32 where p is not negligible.
+// 2^-22 of its value and its argument by 2^-24 |l - top|, a few steps of fp32 where p is not negligible.  Over 131072 x 256
+// fp32 logits p is off by 6.1e-8 of its norm, with expf by 5.9e-8, and the passes take 112 and 68 us, with expf 116 and 69
+// (bf16: 108 and 47, 115 and 51).
 template <int G, int V>
 __device__ __forceinline__ float group_exp(const float (&l)[V], float (&e)[V], float& top) {
   float m = -INFINITY;
@@ -512,8 +514,10 @@ struct RouteBackwardArgs {
 //   normalised:  dl_e = [e in S] w_e (g_e - sum_S w g)          else:  dl_e = p_e ([e in S] g_e - sum_S p g)
 //   balance:     dl_e += db * E / tokens * p_e (f_e - sum_e' p_e' f_e')
 //   z:           dl_e += dz * 2 / tokens * lse * p_e
-// The softmax is formed again from the logits: reading them costs what reading a saved p would.  131072 x 256 fp32: 70 us,
-// 61 % of the copy rate (80 at two blocks an SM); the chosen experts' own terms go through shared memory (by shuffles 77 us).
+// The softmax is formed again from the logits: reading them costs what reading a saved p would.  131072 x 256 fp32: 68 us,
+// 63 % of the copy rate; before the last steps 80 at two blocks an SM and 70 at four, and 77 with the chosen experts' own terms
+// by shuffles in place of shared memory.  A lane's V consecutive values put its 16-byte words V values from its neighbours'
+// and its reads of `mine` into few banks (the same in bf16: 47 %, 32768 x 1024 fp32: 30 %).
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(256, V <= 16 ? 4 : 2)
 route_backward_kernel(const RouteBackwardArgs a) {
@@ -584,7 +588,8 @@ route_backward_kernel(const RouteBackwardArgs a) {
 // Every block owns `chunk` consecutive choices, every warp of it an equal consecutive part.  A block's first row for an
 // expert is what earlier experts hold altogether plus what earlier blocks hold of this one: every block adds up all
 // histograms (they stay in the second-level cache), which costs less than a third launch that would do it once.
-// Bound by latency: 131072 x 8 choices of 256 experts 20 us, 32768 x 4 of 128 10 us (a thread per four experts: 45 and 14).
+// 32768 x 4 choices of 128 experts take 10 us, two launches one after the other; 131072 x 8 of 256 take 21, as every block adds
+// 148 histograms of 256 and a warp ranks its choices 32 at a time (a thread per four experts: 14 and 45).
 __device__ __forceinline__ int read_choice(const void* indices, int is_long, long long i, int experts) {
   const long long e = is_long ? reinterpret_cast<const long long*>(indices)[i] : (long long)reinterpret_cast<const int*>(indices)[i];
   return e >= 0 && e < experts ? (int)e : -1;
@@ -701,7 +706,7 @@ __device__ __forceinline__ void clear_tail(W* rows, long long words, long long f
 }
 
 // One warp per (token, segment of 32 * U words): the token's words are read once and stored top_k times.  Bound by memory:
-// 32768 x 2048 bf16 to four experts 107 us, 96 % of the copy rate.
+// 32768 x 2048 bf16 to four experts 105 us, 97 % of the copy rate.
 template <typename W, int U>
 __global__ void __launch_bounds__(256)
 dispatch_kernel(const W* __restrict__ x, long long x_words, int words, int segments, int tokens, int top_k,
@@ -752,7 +757,7 @@ template <typename T, int N> struct Pack {       // N values of T moved as one w
 };
 
 // out[t] = sum_j weights[t, j] * rows[positions[t, j]], added in fp32 in the order of j; weights null: all one.
-// A warp per (token, segment of 32 * U packs).  Bound by memory: 32768 x 2048 bf16, four choices, 106 us (97 % of the copy
+// A warp per (token, segment of 32 * U packs).  Bound by memory: 32768 x 2048 bf16, four choices, 106 us (96 % of the copy
 // rate); threads over the flattened result instead of warps over rows took 158.
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(256, 2)
@@ -796,8 +801,8 @@ combine_kernel(const T* __restrict__ rows, int width, int segments, int tokens, 
 // drows[positions[t, j]] = weights[t, j] * dout[t],  dweights[t, j] = <dout[t], rows[positions[t, j]]>
 // A token is served by `team` warps of a block (1, 2, 4 or 8) with up to U packs a lane in flight; after the first choice
 // its row of dout comes from the cache, and the dot products end in the block.
-// 32768 tokens x 1152 bf16, two choices: 94 us with two warps of four packs that split a row unevenly, 77 us evenly, 67 us
-// with one warp of five (82 % of the copy rate).  Bound by loads in flight: at 2 blocks an SM instead of 3 or 4 it takes 109.
+// 32768 tokens x 1152 bf16, two choices: 94 us with two warps of four packs that split a row unevenly, 77 us evenly, 64 us
+// with one warp of five (90 % of the copy rate).  Bound by loads in flight: at 2 blocks an SM instead of 3 or 4 it took 109.
 template <typename T, int N, int U>
 __global__ void __launch_bounds__(256, U <= 4 ? 4 : 3)
 combine_backward_kernel(const T* __restrict__ dout, const T* __restrict__ rows, int width, int tokens, int top_k, int team,
@@ -930,7 +935,9 @@ extern "C" int vb_route_forward(const void* logits, int dtype, int tokens, int e
               workspace};
   a.wide = route_wide(logits, stride, experts, lanes, per_lane, dtype == kF32 ? 4 : 2);
   const size_t lists = per_lane > 1 && per_lane <= 16 ? 8 * route_list_words(per_lane) * sizeof(int) : 0;
-  // at most 40 KB
+  // at most 42 KB: 512 experts in 32 lanes of 16 keys
+  static_assert(8 * route_list_words(16) * 4 + 2 * 512 * 4 <= 47 * 1024 && 8 * kMaxExperts * 4 + 2 * kMaxExperts * 4 <= 47 * 1024,
+                "beyond what a kernel has without asking for more");
   const size_t smem = ((size_t)(experts + 3) / 4 * 4 + lanes * per_lane) * 4 + std::max(lists, (size_t)8 * experts * sizeof(float));
   VB_FLOAT_SWITCH(dtype, VB_ROUTE_SWITCH((route_forward_kernel<T, G, V><<<blocks, 256, smem, stream>>>(a))));
   count_launch();
@@ -990,13 +997,14 @@ extern "C" int vb_expert_plan(const void* indices, int is_long, int n, int exper
 }
 
 // Blocks of 8 warps for so many items of a warp.  32 blocks an SM, four times what is resident, even out the tail of long
-// runs: dispatch of 32768 x 2048 bf16 to four experts 113 us at 8 blocks an SM, 107 us (96 % of the copy rate) at 32.
+// runs: dispatch of 32768 x 2048 bf16 to four experts 113 us at 8 blocks an SM, 107 us at 32 in the same run.
 static int row_blocks(long long items) {
   const long long most = items >= 148LL * 32 * 8 ? 148 * 32 : 148 * 8;
   return (int)std::max<long long>(1, std::min<long long>((items + 7) / 8, most));
 }
 // Packs a lane: a whole row (up to 8 a lane) to a warp where that leaves every SM 16 warps, so that all its loads are in
-// flight together, else 2.  32768 x 1152 bf16, two choices: combine 51 us at 2 a lane, 40 us at 5.
+// flight together, else 2.  32768 x 1152 bf16, two choices: combine 52 us at 2 a lane, 45 us at 5; 32768 x 2048, four choices:
+// 120 at 2, 106 at 8.
 static int row_packs(int packs, int tokens) {
   if (tokens < 148 * 16) return 2;
   const int segments = (packs + 255) / 256, per_lane = (packs + segments * 32 - 1) / (segments * 32);

@@ -8,8 +8,10 @@
     rows = experts(rows, plan.offsets)                       # GroupedLinear layers
     x = combine_tokens(rows, routing.weights, plan)          # [..., width]
 
-Nothing waits for the GPU: the row count is ``tokens * top_k`` whatever was chosen, and rows that no choice fills (tokens
-of a padded batch) are zero and lie behind the last expert's.  Results do not depend on the order in which the GPU runs
+The four functions and their gradients never wait for the GPU, and neither does the forward pass of ``GroupedLinear``: the
+row count is ``tokens * top_k`` whatever was chosen, and rows that no choice fills (tokens of a padded batch) are zero and lie
+behind the last expert's.  (``GroupedLinear``'s weight gradient does wait: it reads the offsets on the host, so a training step
+through expert layers cannot be captured into a CUDA graph.)  Results do not depend on the order in which the GPU runs
 its blocks.  CPU tensors take the same path through the PyTorch restatements.  On the GPU the gradients cannot be
 differentiated again, and inputs with forward-mode tangents are refused.
 """
@@ -36,7 +38,11 @@ class Routing(NamedTuple):
 
 
 class ExpertPlan(NamedTuple):
-    """Result of :func:`plan_experts`: where the rows of the experts lie."""
+    """Result of :func:`plan_experts`: where the rows of the experts lie.
+
+    The two belong together: every row below ``offsets[-1]`` is the row of exactly one choice, and on the GPU nothing checks
+    that.  A row that no position names is left unwritten there, in :func:`dispatch_tokens` and in the gradient of
+    :func:`combine_tokens`; to drop a choice, set its index to -1 before planning."""
 
     offsets: torch.Tensor        # int32 [experts + 1]: expert e has the rows offsets[e] .. offsets[e + 1] - 1
     positions: torch.Tensor      # int32 [tokens, top_k]: the row of every choice, -1 for none
@@ -57,8 +63,10 @@ def route_tokens(logits, top_k, *, bias=None, mask=None, normalize=True):
 
     With p the softmax of a token's logits and S its chosen experts, the weights are ``p_e / sum_S p`` (``normalize``) or
     ``p_e``, in fp32 whatever the logits' dtype.  S holds the largest ``fp32(logit) + bias`` (``bias``: optional fp32
-    [experts], it moves the choice and nothing else; +inf counts as the largest number), the lowest index among equals; an expert whose logit is -inf is never
-    chosen, and slots left over get index -1 and weight 0.  ``mask`` (bool, the leading shape) is False for padding:
+    [experts], it moves the choice and nothing else; +inf counts as the largest number), the lowest index among equals; an
+    expert whose logit is -inf is never chosen, and slots left over get index -1 and weight 0.  The bias is added to the
+    logits, which multiplies an expert's p by ``exp(bias)``: one that was trained to be added to p, or to a sigmoid of the
+    logit, chooses other experts here.  ``mask`` (bool, the leading shape) is False for padding:
     those tokens, like tokens with no logit above -inf, choose nothing and enter no sum whatever their logits hold.
 
     ``balance_loss = experts * sum_e f_e P_e`` with f_e the expert's share of all choices (``counts``) and P_e the mean of
